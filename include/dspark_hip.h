@@ -39,7 +39,7 @@ enum {
 
 enum { DSK_F32 = 0, DSK_BF16 = 1 };
 
-enum { DSK_KV_BF16 = 0, DSK_KV_U8 = 1 };
+enum { DSK_KV_BF16 = 0, DSK_KV_U8 = 1, DSK_KV_U4 = 2 };
 
 const char* dsk_last_error(void);
 int dsk_abi_version(void);
@@ -228,6 +228,14 @@ int dsk_w8_embed(const int32_t* ids, int n, const uint8_t* q, const uint16_t* sc
  *   bf16: kv[p][h][t][hd] bf16
  *   u8:   kv[p][h][t][hd] u8 + sb[p][h][t][hd/64] u32 (bf16 scale | bf16 bias << 16),
  *         affine group-64 along head_dim, same rule as dsk_w8_quantize.
+ *   u4:   hd/2 bytes per token and head, sb as u8 with codes 0..15: s = bf16((max - min) / 15) (1 where
+ *         that is not positive), b = bf16(min), a value is bf16(s * c + b). `page` is a multiple of 32.
+ *         Token t, dim d of a page of one head (page * hd / 2 bytes):
+ *           K  byte t * hd/2 + (d/128)*64 + ((d%32)/8)*16 + ((d%128)/32)*4 + (d%8)/2, high half for odd d
+ *           V  byte (t/32)*16*hd + (d/64)*1024 + (d%16 + 16*((t%16)/4))*16 + ((d%64)/32)*8
+ *              + ((t%32)/16)*4 + t%4, high half where d%32 >= 16
+ *         (whole matrix-instruction operands per 16-byte load; MLX's QuantizedKVCache with bits=4 holds
+ *         the same codes row by row, src/mlx_dspark/target.py:36-48).
  * block_table [B, max_pages] int32 maps a row's logical page j to a physical page.
  * seq_lens [B] int32 = tokens cached per row before the call (device memory).
  * ------------------------------------------------------------------------------------- */
@@ -257,6 +265,18 @@ int dsk_qkv_norm_rope_append(const void* qkv, int qkv_splits, int B, int W, int 
                              const int32_t* seq_lens, int pos_offset, const int32_t* block_table,
                              int max_pages, int page, int kv_dtype, void* k_pool, void* v_pool,
                              uint32_t* k_sb, uint32_t* v_sb, uint16_t* q_out, dsk_stream_t stream);
+
+/* Both append entries above write a DSK_KV_U4 pool too (head_dim 128 or 256, 16-byte aligned buffers):
+ * a row then stays float32 from the projection's sum to its code, and is rotated by the exact product
+ * of position and frequency. Tokens at positions beyond the row's block table are dropped.
+ *
+ * dsk_kv_read: positions first[b] + offset + i (i < n) of every row as bf16 rows k_out, v_out
+ * [B, n, nkv, hd], whatever the cache holds them in: the values attention reads (mx.dequantize of a
+ * QuantizedKVCache's state). Rows of positions outside [0, max_pages * page) are left as they were. */
+int dsk_kv_read(const int32_t* first, int offset, int B, int n, int nkv, int hd,
+                const int32_t* block_table, int max_pages, int page, int kv_dtype, const void* k_pool,
+                const void* v_pool, const uint32_t* k_sb, const uint32_t* v_sb, uint16_t* k_out,
+                uint16_t* v_out, dsk_stream_t stream);
 
 /* Attention of W new queries per row over the row's paged KV (already holding the W new
  * tokens at positions seq_lens[b] .. seq_lens[b]+W-1).

@@ -23,6 +23,7 @@
 #include <algorithm>
 
 #include "common.h"
+#include "kv4_entry.h"
 #include "kvrow.h"
 
 namespace dsk {
@@ -1970,6 +1971,10 @@ static int qkv_append_entry(const void* qkv, int qkv_splits, int B, int W, int n
   DSK_REQUIRE(page > 0 && max_pages > 0, "dsk_qkv_rope_append: bad page geometry");
   DSK_REQUIRE(qkv_splits >= 0, "dsk_qkv_rope_append: qkv_splits=%d", qkv_splits);
   DSK_REQUIRE(!x_ssq || qkv_splits > 0, "dsk_qkv_rope_append_rn: the row scale applies to f32 split-K slices");
+  if (kv_dtype == DSK_KV_U4)
+    return kv4_append(qkv, qkv_splits, B, W, nq, nkv, hd, q_norm, k_norm, v_norm, eps, inv_freq, seq_lens, pos_offset,
+                      block_table, max_pages, page, k_pool, v_pool, k_sb, v_sb, q_out, x_ssq, x_tiles, x_eps,
+                      as_stream(stream));
   DSK_REQUIRE(kv_dtype == DSK_KV_BF16 || (kv_dtype == DSK_KV_U8 && k_sb && v_sb),
               "dsk_qkv_rope_append: u8 KV needs scale/bias buffers");
   // many rows: a workgroup per row instead of a wave per head, where that was no slower in a sweep of 1 to

@@ -99,11 +99,13 @@ SIGNATURES: dict[str, tuple] = {
     "dsk_row_logprobs_ws_bytes": (c_size_t, [c_int, c_int64, c_int]),
     "dsk_row_logprobs_ws": (c_int, [c_void_p, c_int64, c_int, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                     c_void_p, c_size_t, c_void_p]),
+    "dsk_kv_read": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p,
+                            c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "dsk_logits_penalize": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
 }
 
 DSK_F32, DSK_BF16 = 0, 1
-DSK_KV_BF16, DSK_KV_U8 = 0, 1
+DSK_KV_BF16, DSK_KV_U8, DSK_KV_U4 = 0, 1, 2
 DSK_EPI_STORE, DSK_EPI_SWIGLU, DSK_EPI_GEGLU, DSK_EPI_PARTIAL, DSK_EPI_RESIDUAL = 0, 1, 2, 3, 4
 
 

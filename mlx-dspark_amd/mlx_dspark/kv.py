@@ -19,7 +19,8 @@ import math
 
 import torch
 
-from .ops import DSK_KV_BF16, DSK_KV_U8
+from . import ops
+from .ops import DSK_KV_BF16, DSK_KV_U4, DSK_KV_U8
 
 
 class LayerView:
@@ -83,16 +84,20 @@ class PagedKVCache(list):
         self.page = page
         self.max_pages = math.ceil(max_ctx / page)
         self.max_ctx = self.max_pages * page
-        self.kv_dtype = DSK_KV_U8 if kv_bits == 8 else DSK_KV_BF16
-        if kv_bits not in (None, 8):
-            raise ValueError(f"kv_bits={kv_bits}: only 8-bit (or None = bf16) KV is supported")
+        if kv_bits not in (None, 4, 8):
+            raise ValueError(f"kv_bits={kv_bits}: only 8-bit and 4-bit (or None = bf16) KV is supported")
+        if kv_bits == 4 and (page % 32 or head_dim not in (128, 256)):
+            raise ValueError(f"4-bit KV needs pages of a multiple of 32 tokens and a head_dim of 128 or 256 "
+                             f"(got {page}, {head_dim})")
+        self.kv_dtype = {None: DSK_KV_BF16, 8: DSK_KV_U8, 4: DSK_KV_U4}[kv_bits]
         self.n_pages = (B + spare_rows) * self.max_pages + spare_pages
         dev = torch.device(device)
-        shape = (self.n_pages, n_kv, page, head_dim)
-        dt = torch.uint8 if self.kv_dtype == DSK_KV_U8 else torch.bfloat16
+        # 4-bit codes: two per byte, in the order dspark_hip.h gives (K by token, V by blocks of 32 tokens)
+        shape = (self.n_pages, n_kv, page, head_dim // 2 if kv_bits == 4 else head_dim)
+        dt = torch.uint8 if kv_bits else torch.bfloat16
         self.k = [torch.zeros(shape, dtype=dt, device=dev) for _ in range(n_layers)]
         self.v = [torch.zeros(shape, dtype=dt, device=dev) for _ in range(n_layers)]
-        if self.kv_dtype == DSK_KV_U8:
+        if kv_bits:
             sbs = (self.n_pages, n_kv, page, head_dim // 64)
             self.k_sb = [torch.zeros(sbs, dtype=torch.int32, device=dev) for _ in range(n_layers)]
             self.v_sb = [torch.zeros(sbs, dtype=torch.int32, device=dev) for _ in range(n_layers)]
@@ -148,10 +153,22 @@ class PagedKVCache(list):
     def layer_args(self, l: int):
         return self.k[l], self.v[l], self.k_sb[l], self.v_sb[l]
 
+    def read(self, layer: int, start: int = 0, n: int | None = None):
+        """(keys, values) of positions start .. start + n - 1 (default: to the shortest row's length) of every
+        row as bf16 [B, n, n_kv, head_dim], whatever the cache holds them in: the reference's
+        ``cache.state`` of a quantized cache, dequantized."""
+        n = min(self.lengths) - int(start) if n is None else int(n)
+        if start < 0 or n < 0 or start + n > self.max_ctx:
+            raise ValueError(f"positions {start} .. {start + n} outside the cache's {self.max_ctx}")
+        k, v, k_sb, v_sb = self.layer_args(layer)
+        first = torch.full((self.B,), int(start), dtype=torch.int32, device=k.device)
+        return ops.kv_read(first, n, self.n_kv, self.head_dim, self.block_table, self.page, self.kv_dtype, k, v, k_sb,
+                           v_sb)
+
     @property
     def nbytes(self) -> int:
         t = sum(x.numel() * x.element_size() for x in self.k + self.v)
-        if self.kv_dtype == DSK_KV_U8:
+        if self.kv_dtype != DSK_KV_BF16:
             t += sum(x.numel() * 4 for x in self.k_sb + self.v_sb)
         return t
 

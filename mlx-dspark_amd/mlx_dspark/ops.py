@@ -16,16 +16,16 @@ import torch
 
 from . import _hip
 from ._hip import (DSK_BF16, DSK_EPI_GEGLU, DSK_EPI_PARTIAL, DSK_EPI_RESIDUAL, DSK_EPI_STORE, DSK_EPI_SWIGLU, DSK_F32,
-                   DSK_KV_BF16, DSK_KV_U8, call, ptr, stream_ptr)
+                   DSK_KV_BF16, DSK_KV_U4, DSK_KV_U8, call, ptr, stream_ptr)
 
 __all__ = [
     "W8Weight", "W8Table", "Workspace", "Packed", "act_pack", "pack", "pack_rn", "w8_gemm", "w8_residual", "w8_embed",
     "w8_dequant", "Rows", "rows_prep", "w8_rows", "rows_rmsnorm", "rows_gated",
-    "qkv_rope_append", "attention", "attention_rows", "attention_rows_split",
+    "qkv_rope_append", "kv_read", "attention", "attention_rows", "attention_rows_split",
     "qkv_attention", "row_logprobs", "accept_greedy", "accept_sample", "sample_rows",
     "argmax_rows", "lens_add",
     "rope_inv_freq", "DSK_EPI_STORE", "DSK_EPI_SWIGLU", "DSK_EPI_GEGLU", "DSK_EPI_PARTIAL", "DSK_KV_BF16",
-    "DSK_KV_U8",
+    "DSK_KV_U8", "DSK_KV_U4",
 ]
 
 
@@ -33,6 +33,13 @@ def _require_cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
             raise ValueError("dspark kernels need device tensors (got a CPU tensor)")
+
+
+def _on_device(t: torch.Tensor) -> None:
+    """A kernel runs on the current device's current stream: refuse tensors of another device."""
+    if t.device.index not in (None, torch.cuda.current_device()):
+        raise ValueError(f"tensors are on {t.device}, the current device is {torch.cuda.current_device()}: call under "
+                         f"torch.cuda.device({t.device.index})")
 
 
 # ----------------------------------------------------------------------------- workspace
@@ -471,6 +478,9 @@ def qkv_rope_append(qkv, B, W, nq, nkv, hd, q_norm, k_norm, eps, inv_freq, seq_l
         qkv = qkv.contiguous().to(torch.bfloat16)
     if q_out is None and nq:
         q_out = torch.empty((B * W, nq * hd), dtype=torch.bfloat16, device=qkv.device)
+    if kv_dtype == DSK_KV_U4:   # 16-byte loads only
+        qkv, q_norm, k_norm, v_norm = (t if t is None or t.data_ptr() % 16 == 0 else t.clone()
+                                       for t in (qkv, q_norm, k_norm, v_norm))
     if x is not None and x.ssq is not None:
         if pos_offset or v_norm is not None:
             raise ValueError("qkv_rope_append: a normed-later input takes no pos_offset / v_norm")
@@ -482,6 +492,30 @@ def qkv_rope_append(qkv, B, W, nq, nkv, hd, q_norm, k_norm, eps, inv_freq, seq_l
          float(eps), ptr(inv_freq), ptr(seq_lens), int(pos_offset), ptr(block_table), block_table.shape[1], page,
          kv_dtype, ptr(k_pool), ptr(v_pool), ptr(k_sb), ptr(v_sb), ptr(q_out), stream_ptr())
     return q_out
+
+
+def kv_read(first, n, nkv, hd, block_table, page, kv_dtype, k_pool, v_pool, k_sb=None, v_sb=None, *, offset=0,
+            k_out=None, v_out=None):
+    """Positions first[b] + offset .. + n - 1 (first int32 [B] on the device) of a paged cache's rows as bf16
+    (k, v) [B, n, nkv, hd], whatever the cache holds them in: the values attention reads. Positions outside
+    the block table leave their rows of k_out / v_out as they were (unset without them)."""
+    B = block_table.shape[0]
+    _require_cuda(first, k_pool)
+    if first.dtype != torch.int32 or first.numel() != B or not first.is_contiguous():
+        raise ValueError(f"kv_read: first must be int32 [{B}]")
+    outs = []
+    for t in (k_out, v_out):
+        if t is None:
+            t = torch.empty((B, n, nkv, hd), dtype=torch.bfloat16, device=k_pool.device)
+        elif t.dtype != torch.bfloat16 or tuple(t.shape) != (B, n, nkv, hd) or not t.is_contiguous():
+            raise ValueError(f"kv_read: outputs must be contiguous bf16 [{B}, {n}, {nkv}, {hd}]")
+        outs.append(t)
+    if n == 0:
+        return tuple(outs)
+    _on_device(k_pool)
+    call("dsk_kv_read", ptr(first), int(offset), B, int(n), nkv, hd, ptr(block_table), block_table.shape[1], page,
+         kv_dtype, ptr(k_pool), ptr(v_pool), ptr(k_sb), ptr(v_sb), ptr(outs[0]), ptr(outs[1]), stream_ptr())
+    return tuple(outs)
 
 
 def attention(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table, page, kv_dtype, k_pool,
