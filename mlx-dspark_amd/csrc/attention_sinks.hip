@@ -1,0 +1,942 @@
+// Attention over a paged KV cache of bf16, 8-bit or 4-bit values with an optional sliding window and the
+// context's first tokens (sinks) visible beside it: decode, verify and prompt passes.
+//
+// Transposed as the other attention kernels are, S^T[key][q] = K . Q^T and O^T[d][q] = V^T . P^T, so a lane
+// owns one query column: lane l (n = l % 16, g = l / 16) holds query n's scores of keys 4 g + r and
+// 16 + 4 g + r of a 32-key block, which are its 8 items of the P operand, and V^T comes in that key order.
+// Keys are visited in aligned blocks of 32: first the blocks that hold sinks, then those from the window's
+// start (or 0) to the last key. Scores, running maximum, sum and output are float32; a probability enters
+// the P.V product as two bf16 terms (within 2^-17 of it).
+//
+// The maximum moves only when a score passes it by 2^8: below that the exponentials stay in float32's
+// range and nothing is lost, and a block costs one vote instead of two lane exchanges and a rescale.
+#include <algorithm>
+
+#include "common.h"
+#include "kv4.h"
+
+namespace dsk {
+
+struct SinkArgs {
+  const uint16_t* q;  // [B*W][nq*HD]
+  int B, W, nq, nkv, G, R;  // R = W * G query rows per (row b, kv head)
+  float scale, softcap;
+  int causal, window, sinks;  // window 0: none
+  const int32_t* seq_lens;
+  const int32_t* block_table;
+  int max_pages, page;
+  const void *k_pool, *v_pool;
+  const uint32_t *k_sb, *v_sb;
+  uint16_t* out;
+  int out_packed;
+  int groups;    // row groups of a (row b, kv head), one workgroup each per split
+  int grows;     // rows per group
+  int slots;     // splits on the grid per kv head: balanced over the rows' lengths (groups == 1), or
+                 // nsplit for each row and group
+  int nsplit, balanced;
+  float* part_o;   // [slot][kv head][R][HD] unnormalised outputs
+  float* part_ml;  // [slot][kv head][R][2] running maximum (of scores times c2) and sum
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kMaxSlack = 8.0f;   // how far (log2) a score may pass the running maximum
+constexpr int kMinSplitBlocks = 4;  // 32-key blocks per split at least: one per wave
+constexpr int kBalancedRows = 64;   // rows whose lengths a workgroup reads to place its split
+
+// The 32-key blocks that query tokens i0 .. i1 of row b look at.
+struct KeyPlan {
+  int off, j_beg, j_end;  // cached keys; first key of the window range, end of the keys
+  int beg, nA, T;         // sink blocks 0 .. nA - 1 sit at 32 v, the others at beg + 32 (v - nA); T in all
+  __device__ __forceinline__ int base(int v) const { return v < nA ? 32 * v : beg + 32 * (v - nA); }
+};
+__device__ __forceinline__ KeyPlan key_plan(const SinkArgs& a, int len, int i0, int i1) {
+  KeyPlan p;
+  p.off = max(len, 0);
+  const int Lk = (int)min((int64_t)p.off + a.W, (int64_t)a.max_pages * a.page);
+  const bool windowed = a.causal && a.window > 0;
+  p.j_end = a.causal ? min(Lk, p.off + i1 + 1) : Lk;
+  p.j_beg = windowed ? min(p.j_end, max(0, p.off + i0 - a.window + 1)) : 0;
+  p.beg = p.j_beg & ~31;
+  p.nA = windowed ? (min(a.sinks, p.j_end) + 31) / 32 : 0;
+  if (32 * p.nA >= p.beg) p.nA = p.beg = 0;  // the two ranges meet
+  p.T = p.nA + (p.j_end - p.beg + 31) / 32;
+  return p;
+}
+__device__ __forceinline__ int round4(int x) { return (x + 3) & ~3; }
+
+// Which split a workgroup runs: the row b, its slot of the partial buffers, its blocks [v0, v1) and the
+// number of splits that the row (and group) has. Balanced: blocks per split from the rows' summed lengths, so that rows
+// of very different lengths load the chip evenly. live == 0: nothing to do.
+struct SplitTask {
+  int b, slot, v0, v1, live;
+  KeyPlan p;
+};
+__device__ __forceinline__ int balanced_blocks(const SinkArgs& a) {
+  int total = 0;
+  for (int b = 0; b < a.B; ++b) total += key_plan(a, a.seq_lens[b], 0, a.W - 1).T;
+  return max(kMinSplitBlocks, round4((total + a.slots - a.B - 1) / (a.slots - a.B)));
+}
+__device__ __forceinline__ SplitTask split_task(const SinkArgs& a, int slot, int group) {
+  SplitTask t;
+  t.slot = slot;
+  t.live = 0;
+  if (a.balanced) {
+    const int bps = balanced_blocks(a);
+    int first = 0;
+    for (int b = 0; b < a.B; ++b) {
+      const KeyPlan p = key_plan(a, a.seq_lens[b], 0, a.W - 1);
+      const int live = max(1, (p.T + bps - 1) / bps);
+      if (slot < first + live) {
+        t.b = b;
+        t.p = p;
+        t.live = live;
+        t.v0 = (slot - first) * bps;
+        t.v1 = min(p.T, t.v0 + bps);
+        break;
+      }
+      first += live;
+    }
+    return t;
+  }
+  t.b = slot / a.nsplit;
+  t.p = key_plan(a, a.seq_lens[t.b], group * a.grows / a.G, (min(a.R, (group + 1) * a.grows) - 1) / a.G);
+  const int bps = max(kMinSplitBlocks, round4((t.p.T + a.nsplit - 1) / a.nsplit));
+  const int s = slot % a.nsplit, live = max(1, (t.p.T + bps - 1) / bps);
+  if (s < live) t.live = live;
+  t.v0 = s * bps;
+  t.v1 = min(t.p.T, t.v0 + bps);
+  return t;
+}
+
+// The keys a query at position pos sees: j <= last and (j >= first or j < sinks). Selects throughout: with
+// branches here the compiler has dropped the masking of a score in a branch's far side.
+struct Sight {
+  int first, last, sinks;
+  __device__ __forceinline__ bool sees(int j) const { return bool((int)(j <= last) & ((int)(j >= first) | (int)(j < sinks))); }
+};
+__device__ __forceinline__ Sight sight(const SinkArgs& a, const KeyPlan& p, int pos) {
+  const bool windowed = a.causal && a.window > 0;
+  return Sight{windowed ? pos - a.window + 1 : 0, a.causal ? min(p.j_end - 1, pos) : p.j_end - 1, windowed ? a.sinks : 0};
+}
+// whether block [j, j + 31] needs no mask for queries at positions lo .. hi, and whether none of them sees it
+__device__ __forceinline__ bool block_open(const SinkArgs& a, const KeyPlan& p, int j, int lo, int hi) {
+  if (j + 31 >= p.j_end) return false;
+  if (!a.causal) return true;
+  return j + 31 <= lo && (a.window <= 0 || j > hi - a.window || j + 31 < a.sinks);
+}
+__device__ __forceinline__ bool block_shut(const SinkArgs& a, int j, int lo, int hi) {
+  return a.causal && (j > hi || (a.window > 0 && j + 31 <= lo - a.window && j >= a.sinks));
+}
+// whether no query of the plan sees key j: what stands there (the slots behind the last key, expired keys)
+// is kept out of the P.V product, where a probability of 0 would not undo an infinity or a NaN
+__device__ __forceinline__ bool key_dead(const SinkArgs& a, const KeyPlan& p, int j) {
+  return bool((int)(j >= p.j_end) | ((int)(j < p.j_beg) & (int)(j >= a.sinks)));
+}
+
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ bool nonfinite2(uint32_t w) {
+  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+__device__ __forceinline__ int64_t sink_out_index(const SinkArgs& a, int HD, int b, int r, int kvh, int d) {
+  const int64_t m = (int64_t)b * a.W + r / a.G, k = (int64_t)(kvh * a.G + r % a.G) * HD + d;
+  return a.out_packed ? apack_index(m, k, (int64_t)a.nq * HD / 64) : m * a.nq * HD + k;
+}
+
+// The running state of one tile of 16 queries over the keys seen so far.
+template <int HD>
+struct Tile {
+  float m, l;  // maximum (times c2) of the lane's query; the lane's own keys' sum
+  f32x4 o[HD / 16];
+  __device__ __forceinline__ void clear() {
+    m = -__builtin_inff();
+    l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0, 0, 0, 0};
+  }
+  // scores -> probabilities in place
+  template <int NKT>
+  __device__ __forceinline__ void soften(f32x4 (&st)[NKT], float c2) {
+    float mx = -__builtin_inff();
+#pragma unroll
+    for (int t = 0; t < NKT; ++t) mx = fmaxf(mx, fmaxf(fmaxf(st[t][0], st[t][1]), fmaxf(st[t][2], st[t][3])));
+    if (__any(mx * c2 > m + kMaxSlack)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float mn = fmaxf(m, mx * c2);
+      const float alpha = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) o[d] *= alpha;
+    }
+    const float mb = m == -__builtin_inff() ? 0.0f : m;  // a row with no visible key yet: exp2(-inf) = 0
+#pragma unroll
+    for (int t = 0; t < NKT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        st[t][r] = __builtin_amdgcn_exp2f(fmaf(st[t][r], c2, -mb));
+        l += st[t][r];
+      }
+  }
+  // the two bf16 terms of 8 probabilities (tiles t, t + 1 of a 32-key block)
+  static __device__ __forceinline__ void terms(const f32x4& a, const f32x4& b, u32x4& hi, u32x4& lo) {
+    uint32_t h[4], w[4];
+    split2_bf16x2(a[0], a[1], h[0], w[0]);
+    split2_bf16x2(a[2], a[3], h[1], w[1]);
+    split2_bf16x2(b[0], b[1], h[2], w[2]);
+    split2_bf16x2(b[2], b[3], h[3], w[3]);
+    hi = u32x4{h[0], h[1], h[2], h[3]};
+    lo = u32x4{w[0], w[1], w[2], w[3]};
+  }
+  // O^T += V^T . P^T where a key that some query does not see holds an infinity or a NaN: key by key, each
+  // kept out of the queries that do not see it
+  template <class VF>
+  __device__ __forceinline__ void add_guarded(const Sight& see, int base, int lane, u32x4 hi, u32x4 lo, VF vf) {
+#pragma unroll 1
+    for (int k = 0; k < 32; ++k) {
+      const int e = (k / 16) * 4 + k % 4;
+      const bool mine = (lane >> 4) == (k % 16) / 4, vis = see.sees(base + k);
+      u32x4 keep;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) keep[w] = mine && w == e / 2 ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) {
+        const u32x4 v = vf(d) & keep;
+        const f32x4 t = mfma16(v, lo, mfma16(v, hi, o[d]));
+        o[d] = vis ? t : o[d];
+      }
+    }
+  }
+};
+
+// masks of a 32-key block's (or two blocks') scores: lane holds keys base + 16 t + 4 g + r
+template <int NKT>
+__device__ __forceinline__ void mask_scores(const Sight& see, f32x4 (&st)[NKT], int t0, int base, int g) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    f32x4 x = st[t0 + t];
+    const int j = base + 16 * t + 4 * g;
+    x = f32x4{see.sees(j) ? x[0] : -__builtin_inff(), see.sees(j + 1) ? x[1] : -__builtin_inff(),
+              see.sees(j + 2) ? x[2] : -__builtin_inff(), see.sees(j + 3) ? x[3] : -__builtin_inff()};
+    st[t0 + t] = x;
+  }
+}
+
+// the words of bf16(s c + b) of 8 consecutive dims of an 8-bit row
+__device__ __forceinline__ u32x4 kv8_row8(uint2 r, uint32_t z) {
+  const float s = bits_f32(z << 16), b = bits_f32(z & 0xffff0000u);
+  u32x4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t two = (e < 2 ? r.x : r.y) >> (16 * (e & 1));
+    w[e] = pack_bf16x2(fmaf(s, (float)(two & 255), b), fmaf(s, (float)((two >> 8) & 255), b));
+  }
+  return w;
+}
+
+// ----------------------------------------------------------------------------- K and V of a block
+// One wave's loads of a 32-key block, kept raw until they are used (so the next block's are in flight
+// meanwhile), and the operands they become.
+// K: u32x4 per 16-key tile and 32-dim step (A operand of the score product).
+template <int HD, int KVT>
+struct KRaw {
+  u32x4 q[2][KVT == DSK_KV_BF16 ? HD / 32 : (KVT == DSK_KV_U8 ? HD / 64 : HD / 128)];
+  uint32_t sb[2][KVT == DSK_KV_BF16 ? 1 : HD / 64];
+  // tok: pool token of the block's first key
+  __device__ __forceinline__ void load(const SinkArgs& a, uint32_t tok, int lane) {
+    const int n = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int64_t row = (int64_t)tok + 16 * t + n;
+      if constexpr (KVT == DSK_KV_BF16) {
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(a.k_pool) + row * HD + 8 * g;
+#pragma unroll
+        for (int s = 0; s < HD / 32; ++s) q[t][s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
+      } else if constexpr (KVT == DSK_KV_U8) {
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(a.k_pool) + row * HD + 8 * g;
+#pragma unroll
+        for (int s = 0; s < HD / 64; ++s) {
+          const uint2 x = *reinterpret_cast<const uint2*>(src + 64 * s), y = *reinterpret_cast<const uint2*>(src + 64 * s + 32);
+          q[t][s] = u32x4{x.x, x.y, y.x, y.y};
+        }
+      } else {
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(a.k_pool) + row * (HD / 2) + 16 * g;
+#pragma unroll
+        for (int s = 0; s < HD / 128; ++s) q[t][s] = *reinterpret_cast<const u32x4*>(src + 64 * s);
+      }
+      if constexpr (KVT != DSK_KV_BF16) {
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c) sb[t][c] = a.k_sb[row * (HD / 64) + c];
+      }
+    }
+  }
+  __device__ __forceinline__ u32x4 operand(int t, int s) const {
+    if constexpr (KVT == DSK_KV_BF16) return q[t][s];
+    else if constexpr (KVT == DSK_KV_U8)
+      return kv8_row8(s & 1 ? uint2{q[t][s / 2][2], q[t][s / 2][3]} : uint2{q[t][s / 2][0], q[t][s / 2][1]}, sb[t][s / 2]);
+    else return kv4_row8(q[t][s / 4][s % 4], kv4_scale(sb[t][s / 2]));
+  }
+};
+
+// V operands (d tile, lane) in LDS: 16 bytes per lane, a pad after each lane group spreads the transposing
+// writes of row-major caches over the banks
+constexpr int kVGroup = 256 + 16, kVTile = 4 * kVGroup;  // bytes per lane group, per 16-dim tile
+
+// 4-bit V of one 64-dim chunk c of a block: four d tiles' operands from one 16-byte load per lane
+template <int HD>
+struct V4Raw {
+  u32x4 q;
+  uint32_t sb[8];
+  __device__ __forceinline__ void load(const SinkArgs& a, uint32_t tok, int c, int lane) {
+    q = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint8_t*>(a.v_pool) + (int64_t)tok * (HD / 2) + c * 1024 + lane * 16);
+    const uint32_t* src = a.v_sb + ((int64_t)tok + 4 * (lane >> 4)) * (HD / 64) + c;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sb[e] = src[(16 * (e / 4) + e % 4) * (HD / 64)];
+  }
+  // d tiles 4 c + 2 p + h; dead keys' words cleared before
+  __device__ __forceinline__ void operands(u32x4 (&v)[4]) const {
+    Kv4Scale z[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] = kv4_scale(sb[e]);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      uint32_t lo[2][2], hi[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) kv4_col4(q[2 * p + u], z + 4 * u, lo[u], hi[u]);
+      v[2 * p] = u32x4{lo[0][0], lo[0][1], lo[1][0], lo[1][1]};
+      v[2 * p + 1] = u32x4{hi[0][0], hi[0][1], hi[1][0], hi[1][1]};
+    }
+  }
+  __device__ __forceinline__ void drop_dead(const SinkArgs& a, const KeyPlan& p, int base, int lane) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      sb[e] = key_dead(a, p, base + 16 * (e / 4) + 4 * (lane >> 4) + e % 4) ? 0u : sb[e];
+  }
+};
+
+// row-major V (bf16, 8-bit): 4 keys x 8 dims, transposed on their way into the operand order in LDS
+template <int HD, int KVT>
+struct VRowsRaw {
+  u32x4 q[4];
+  uint32_t sb[4];
+  // quad: keys 4 quad .. + 3 of the block, ch: dims 8 ch .. + 7
+  __device__ __forceinline__ void load(const SinkArgs& a, uint32_t tok, int quad, int ch) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t row = (int64_t)tok + 4 * quad + r;
+      if constexpr (KVT == DSK_KV_BF16) {
+        q[r] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(a.v_pool) + row * HD + 8 * ch);
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(a.v_pool) + row * HD + 8 * ch);
+        q[r] = u32x4{x.x, x.y, 0, 0};
+        sb[r] = a.v_sb[row * (HD / 64) + ch / 8];
+      }
+    }
+  }
+  // base: the block's first key; dst: the block's operands in LDS
+  __device__ __forceinline__ void store(const SinkArgs& a, const KeyPlan& p, int base, int quad, int ch, bool check,
+                                        uint8_t* dst) const {
+    u32x4 w[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if constexpr (KVT == DSK_KV_BF16) w[r] = q[r];
+      else w[r] = kv8_row8(uint2{q[r][0], q[r][1]}, sb[r]);
+      const uint32_t keep = check && key_dead(a, p, base + 4 * quad + r) ? 0u : ~0u;
+      w[r] &= u32x4{keep, keep, keep, keep};
+    }
+    uint8_t* o = dst + (ch / 2) * kVTile + (quad % 4) * kVGroup + (ch % 2) * 128 + (quad / 4) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+      *reinterpret_cast<uint2*>(o + 16 * e) = uint2{__builtin_amdgcn_perm(w[1][e / 2], w[0][e / 2], sel),
+                                                    __builtin_amdgcn_perm(w[3][e / 2], w[2][e / 2], sel)};
+    }
+  }
+};
+
+__device__ __forceinline__ u32x4 v_operand(const uint8_t* blk, int d, int lane) {
+  return *reinterpret_cast<const u32x4*>(blk + d * kVTile + (lane >> 4) * kVGroup + (lane & 15) * 16);
+}
+
+// ----------------------------------------------------------------------------- few query rows
+// One tile of 16 query rows per workgroup; its split's blocks go round its four waves, each with a running
+// state of its own, merged in LDS at the end. No barrier before that: a wave turns its own loads into its
+// own operands (4-bit V lies in operand order; row-major V is transposed through the wave's LDS).
+// Page ids of 64 blocks are loaded at once, one per lane.
+template <int HD, int KVT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 4))) void attention_tile_kernel(SinkArgs a) {
+  constexpr int KS = HD / 32, DT = HD / 16, NI = HD / 128 * 2;  // NI: (quad, chunk) items per lane
+  constexpr bool kRows = KVT != DSK_KV_U4;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kRows && 4 * DT * kVTile > 4 * DT * 1024 ? 4 * DT * kVTile : 4 * DT * 1024];
+  __shared__ float2 wml[4][16];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  const int kvh = blockIdx.x % a.nkv, group = blockIdx.y;
+  const SplitTask t = split_task(a, blockIdx.x / a.nkv, group);
+  if (t.live == 0) return;
+  const KeyPlan& p = t.p;
+  const int r0 = group * a.grows, r = r0 + n, rc = min(r, a.R - 1);
+  const int pos = p.off + rc / a.G, pos_lo = p.off + r0 / a.G, pos_hi = p.off + (min(r0 + 16, a.R) - 1) / a.G;
+  const float c2 = (a.softcap > 0.0f ? 1.0f : a.scale) * kLog2e;
+  const Sight see = sight(a, p, pos);
+
+  const int nblk = t.v1 > t.v0 + wv ? (t.v1 - t.v0 - wv + 3) / 4 : 0;  // this wave's blocks v0 + wv + 4 i
+  uint32_t toks = 0;  // lane l: pool token of block i = (i0 & ~63) + l
+  auto find_tokens = [&](int i) {
+    const int base = p.base(min(t.v0 + wv + 4 * (i + lane), t.v1 - 1));
+    const int pg = a.block_table[(int64_t)t.b * a.max_pages + base / a.page];
+    toks = ((uint32_t)pg * a.nkv + kvh) * a.page + base % a.page;
+  };
+  auto token = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane(toks, i & 63); };
+
+  KRaw<HD, KVT> k;
+  V4Raw<HD> v4[kRows ? 1 : HD / 64];
+  VRowsRaw<HD, KVT> vr[kRows ? NI : 1];
+  auto load_v = [&](uint32_t tok) {
+    if constexpr (kRows) {
+#pragma unroll
+      for (int u = 0; u < NI; ++u) {
+        const int i = lane + 64 * u;
+        vr[u].load(a, tok, (i >> 1) % 8, (i & 1) + 2 * (i >> 4));
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < HD / 64; ++c) v4[c].load(a, tok, c, lane);
+    }
+  };
+  if (nblk > 0) {
+    find_tokens(0);
+    k.load(a, token(0), lane);
+    load_v(token(0));
+  }
+  u32x4 qf[KS];
+  {
+    const uint16_t* src = a.q + ((int64_t)(t.b * a.W + rc / a.G) * a.nq + kvh * a.G + rc % a.G) * HD + 8 * g;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
+  }
+  Tile<HD> tile;
+  tile.clear();
+  uint8_t* vlds = lds + wv * DT * kVTile;
+#pragma unroll 1
+  for (int i = 0; i < nblk; ++i) {
+    const int base = p.base(t.v0 + wv + 4 * i);
+    const bool open = block_open(a, p, base, pos_lo, pos_hi);
+    f32x4 st[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) st[u] = mfma16(k.operand(u, s), qf[s], st[u]);
+    const bool more = i + 1 < nblk;
+    if (more && ((i + 1) & 63) == 0) find_tokens(i + 1);
+    if (more) k.load(a, token(i + 1), lane);
+    if (a.softcap > 0.0f) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st[u][e] = tanhf(st[u][e] * a.scale / a.softcap) * a.softcap;
+    }
+    if (!open) mask_scores(see, st, 0, base, g);
+    tile.soften(st, c2);
+    u32x4 hi, lo;
+    Tile<HD>::terms(st[0], st[1], hi, lo);
+    u32x4 vf[kRows ? 1 : DT];
+    if constexpr (kRows) {
+#pragma unroll
+      for (int u = 0; u < NI; ++u) {
+        const int it = lane + 64 * u;
+        vr[u].store(a, p, base, (it >> 1) % 8, (it & 1) + 2 * (it >> 4), !open, vlds);
+      }
+      asm volatile("" ::: "memory");  // a wave's LDS accesses run in order; keep the compiler's order too
+    } else {
+#pragma unroll
+      for (int c = 0; c < HD / 64; ++c) {
+        if (!open) v4[c].drop_dead(a, p, base, lane);
+        u32x4 x[4];
+        v4[c].operands(x);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) vf[kRows ? 0 : 4 * c + d] = x[d];
+      }
+    }
+    if (more) load_v(token(i + 1));
+    auto operand = [&](int d) {
+      if constexpr (kRows) return v_operand(vlds, d, lane);
+      else return vf[kRows ? 0 : d];
+    };
+    bool guarded = false;
+    if (!open) {
+      bool bad = false;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const u32x4 x = operand(d);
+        bad |= nonfinite2(x[0]) || nonfinite2(x[1]) || nonfinite2(x[2]) || nonfinite2(x[3]);
+      }
+      guarded = __any(bad);
+    }
+    if (guarded) {
+      tile.add_guarded(see, base, lane, hi, lo, operand);
+    } else {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const u32x4 x = operand(d);
+        tile.o[d] = mfma16(x, lo, mfma16(x, hi, tile.o[d]));
+      }
+    }
+    if constexpr (kRows) asm volatile("" ::: "memory");
+  }
+  float l = tile.l;
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+
+  // ---- the four waves' states merged, each wave a quarter of the d tiles
+  __syncthreads();
+  f32x4* mo = reinterpret_cast<f32x4*>(lds);  // [wave][d tile][lane]
+#pragma unroll
+  for (int d = 0; d < DT; ++d) mo[(wv * DT + d) * 64 + lane] = tile.o[d];
+  if (g == 0) wml[wv][n] = float2{tile.m, l};
+  __syncthreads();
+  float M = -__builtin_inff(), L = 0.0f, wq[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) M = fmaxf(M, wml[w][n].x);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    wq[w] = wml[w][n].x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(wml[w][n].x - M);
+    L += wq[w] * wml[w][n].y;
+  }
+  if (r >= a.R) return;
+  const bool whole = t.live == 1;
+  const float inv = L != 0.0f ? 1.0f / L : 0.0f;  // no visible key: zeros; a NaN sum stays NaN
+#pragma unroll
+  for (int dd = 0; dd < DT / 4; ++dd) {
+    const int d = wv * (DT / 4) + dd;
+    f32x4 s = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      if (wq[w] != 0.0f) s += mo[(w * DT + d) * 64 + lane] * wq[w];
+    if (whole) {
+      s *= inv;
+      *reinterpret_cast<uint2*>(a.out + sink_out_index(a, HD, t.b, r, kvh, d * 16 + 4 * g)) =
+          uint2{pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3])};
+    } else {
+      *reinterpret_cast<f32x4*>(a.part_o + (((int64_t)t.slot * a.nkv + kvh) * a.R + r) * HD + d * 16 + 4 * g) = s;
+    }
+  }
+  if (!whole && wv == 0 && g == 0)
+    *reinterpret_cast<float2*>(a.part_ml + (((int64_t)t.slot * a.nkv + kvh) * a.R + r) * 2) = float2{M, L};
+}
+
+// ----------------------------------------------------------------------------- many query rows
+// NW waves of TPW tiles share each chunk of keys: it is loaded and turned into operands once, into one of
+// two LDS buffers, while the other is scored (one barrier per chunk; the chunk after is in flight). Chunks
+// are 64 keys at head_dim 128 and 32 at 256, so a buffer is 33 KB: two workgroups of four waves fit a CU.
+template <int HD> constexpr int kChunkBlocks = HD == 128 ? 2 : 1;
+
+template <int HD, int KVT, int NW, int TPW>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_block_kernel(SinkArgs a) {
+  constexpr int KS = HD / 32, DT = HD / 16, NB = kChunkBlocks<HD>, NKT = 2 * NB;
+  constexpr bool kRows = KVT != DSK_KV_U4;
+  constexpr int kKBytes = NKT * KS * 1024, kVBytes = NB * DT * kVTile;
+  __shared__ __attribute__((aligned(16))) uint8_t kbuf[2][kKBytes];
+  __shared__ __attribute__((aligned(16))) uint8_t vbuf[2][kVBytes];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  const int w4 = wv & 3;
+  const bool do_k = NW == 4 || wv < 4, do_v = NW == 4 || wv >= 4;
+  const int kvh = blockIdx.x % a.nkv, group = a.groups - 1 - (int)blockIdx.y;  // the groups with the most keys first
+  const SplitTask t = split_task(a, blockIdx.x / a.nkv, group);
+  if (t.live == 0) return;
+  const KeyPlan& p = t.p;
+  const int r0 = group * a.grows + wv * TPW * 16;
+  const bool wave_live = r0 < a.R;
+  const int pos_lo = p.off + min(r0, a.R - 1) / a.G, pos_hi = p.off + (min(r0 + TPW * 16, a.R) - 1) / a.G;
+  const float c2 = (a.softcap > 0.0f ? 1.0f : a.scale) * kLog2e;
+  const int nch = t.v1 > t.v0 ? (t.v1 - t.v0 + NB - 1) / NB : 0;
+
+  // this thread's pieces of a chunk: K units of (block, tile[, half]) and V units of (block, chunk) for 4-bit
+  // codes; 4 K tiles of 16 x 32 and 4 keys x 8 dims of V for rows
+  constexpr int kUnits = 4;
+  u32x4 kq[kRows ? kUnits : 1];
+  uint32_t ksb[kRows ? kUnits : 2];
+  V4Raw<HD> v4;
+  VRowsRaw<HD, KVT> vr;
+  uint32_t tok_next[NB];  // tokens of the chunk to issue next
+  auto find = [&](int c) {
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      const int base = p.base(min(t.v0 + c * NB + u, t.v1 - 1));
+      const int pg = a.block_table[(int64_t)t.b * a.max_pages + base / a.page];
+      tok_next[u] = ((uint32_t)pg * a.nkv + kvh) * a.page + base % a.page;
+    }
+  };
+  // U4 K unit w4: tile w4 (head_dim 128: of 64 keys), or tile w4 / 2, half w4 % 2 (256); V unit: chunk w4 % (HD / 64) of block w4 / (HD / 64)
+  constexpr int kHalves = HD / 128;
+  const int kt = w4 / kHalves, kh = w4 % kHalves, vb = w4 / (HD / 64), vc = w4 % (HD / 64);
+  const int item = w4 * 64 + lane, vq = (item >> 1) % 8, vch = (item & 1) + 2 * ((item >> 4) % DT), vblk = (item >> 4) / DT;
+  auto issue = [&]() {
+    if (do_k) {
+      if constexpr (kRows) {
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+          const int id = w4 * kUnits + u, kt2 = id / KS, s = id % KS;  // tile, step
+          const int64_t row = (int64_t)tok_next[kt2 / 2] + 16 * (kt2 % 2) + n;
+          if constexpr (KVT == DSK_KV_BF16) {
+            kq[u] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(a.k_pool) + row * HD + 32 * s + 8 * g);
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(a.k_pool) + row * HD + 32 * s + 8 * g);
+            kq[u] = u32x4{x.x, x.y, 0, 0};
+            ksb[u] = a.k_sb[row * (HD / 64) + s / 2];
+          }
+        }
+      } else {
+        const int64_t row = (int64_t)tok_next[kt / 2] + 16 * (kt % 2) + n;
+        kq[0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint8_t*>(a.k_pool) + row * (HD / 2) + 64 * kh + 16 * g);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) ksb[c] = a.k_sb[row * (HD / 64) + 2 * kh + c];
+      }
+    }
+    if (do_v) {
+      if constexpr (kRows) vr.load(a, tok_next[vblk], vq, vch);
+      else v4.load(a, tok_next[vb], vc, lane);
+    }
+  };
+  auto stage = [&](int buf, int c) {
+    if (do_k) {
+      if constexpr (kRows) {
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+          u32x4 w = kq[u];
+          if constexpr (KVT == DSK_KV_U8) w = kv8_row8(uint2{kq[u][0], kq[u][1]}, ksb[u]);
+          *reinterpret_cast<u32x4*>(&kbuf[buf][(w4 * kUnits + u) * 1024 + lane * 16]) = w;
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          *reinterpret_cast<u32x4*>(&kbuf[buf][(kt * KS + 4 * kh + s) * 1024 + lane * 16]) = kv4_row8(kq[0][s], kv4_scale(ksb[s / 2]));
+      }
+    }
+    if (do_v) {
+      const int blk = kRows ? vblk : vb, v = t.v0 + c * NB + blk;
+      const int base = v < t.v1 ? p.base(v) : 0x40000000;  // past the split: every key dead
+      const bool check = base + 31 >= p.j_end || base < p.j_beg;
+      if constexpr (kRows) {
+        vr.store(a, p, base, vq, vch, check, &vbuf[buf][blk * DT * kVTile]);
+      } else {
+        if (check) v4.drop_dead(a, p, base, lane);
+        u32x4 x[4];
+        v4.operands(x);
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+          *reinterpret_cast<u32x4*>(&vbuf[buf][(blk * DT + 4 * vc + d) * kVTile + g * kVGroup + n * 16]) = x[d];
+      }
+    }
+  };
+
+  u32x4 qf[TPW][KS];
+  Sight see[TPW];
+#pragma unroll
+  for (int u = 0; u < TPW; ++u) {
+    const int rc = min(r0 + 16 * u + n, a.R - 1);
+    see[u] = sight(a, p, p.off + rc / a.G);
+    const uint16_t* src = a.q + ((int64_t)(t.b * a.W + rc / a.G) * a.nq + kvh * a.G + rc % a.G) * HD + 8 * g;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[u][s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
+  }
+  Tile<HD> tile[TPW];
+#pragma unroll
+  for (int u = 0; u < TPW; ++u) tile[u].clear();
+
+  auto compute = [&](int buf, int c) {
+    int base[NB];
+    bool open = true, shut = true;
+#pragma unroll
+    for (int x = 0; x < NB; ++x) {
+      const int v = t.v0 + c * NB + x;
+      base[x] = v < t.v1 ? p.base(v) : 0x40000000;
+      open &= block_open(a, p, base[x], pos_lo, pos_hi);
+      shut &= v >= t.v1 || block_shut(a, base[x], pos_lo, pos_hi);
+    }
+    if (shut || !wave_live) return;
+    f32x4 st[TPW][NKT];
+#pragma unroll
+    for (int u = 0; u < TPW; ++u)
+#pragma unroll
+      for (int x = 0; x < NKT; ++x) st[u][x] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int x = 0; x < NKT; ++x) {
+        const u32x4 kf = *reinterpret_cast<const u32x4*>(&kbuf[buf][(x * KS + s) * 1024 + lane * 16]);
+#pragma unroll
+        for (int u = 0; u < TPW; ++u) st[u][x] = mfma16(kf, qf[u][s], st[u][x]);
+      }
+    u32x4 hi[TPW][NB], lo[TPW][NB];
+#pragma unroll
+    for (int u = 0; u < TPW; ++u) {
+      if (a.softcap > 0.0f) {
+#pragma unroll
+        for (int x = 0; x < NKT; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) st[u][x][e] = tanhf(st[u][x][e] * a.scale / a.softcap) * a.softcap;
+      }
+      if (!open) {
+#pragma unroll
+        for (int x = 0; x < NB; ++x) mask_scores(see[u], st[u], 2 * x, base[x], g);
+      }
+      tile[u].soften(st[u], c2);
+#pragma unroll
+      for (int x = 0; x < NB; ++x) Tile<HD>::terms(st[u][2 * x], st[u][2 * x + 1], hi[u][x], lo[u][x]);
+    }
+#pragma unroll
+    for (int x = 0; x < NB; ++x) {
+      const uint8_t* vb8 = &vbuf[buf][x * DT * kVTile];
+      auto operand = [&](int d) { return v_operand(vb8, d, lane); };
+      if (!open) {
+        bool bad = false;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const u32x4 w = operand(d);
+          bad |= nonfinite2(w[0]) || nonfinite2(w[1]) || nonfinite2(w[2]) || nonfinite2(w[3]);
+        }
+        if (__any(bad)) {
+#pragma unroll
+          for (int u = 0; u < TPW; ++u) tile[u].add_guarded(see[u], base[x], lane, hi[u][x], lo[u][x], operand);
+          continue;
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const u32x4 w = operand(d);
+#pragma unroll
+        for (int u = 0; u < TPW; ++u) tile[u].o[d] = mfma16(w, hi[u][x], tile[u].o[d]);
+#pragma unroll
+        for (int u = 0; u < TPW; ++u) tile[u].o[d] = mfma16(w, lo[u][x], tile[u].o[d]);
+      }
+    }
+  };
+
+  if (nch > 0) {
+    find(0);
+    issue();
+    if (nch > 1) find(1);
+    stage(0, 0);
+    if (nch > 1) issue();
+    if (nch > 2) find(2);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int c = 0; c < nch; ++c) {
+    compute(c & 1, c);
+    if (c + 1 < nch) {
+      // the other buffer was last read for chunk c - 1, before the last barrier
+      stage((c + 1) & 1, c + 1);
+      if (c + 2 < nch) issue();
+      if (c + 3 < nch) find(c + 3);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int u = 0; u < TPW; ++u) {
+    float l = tile[u].l;
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    const int r = r0 + 16 * u + n;
+    if (r >= a.R) continue;
+    if (t.live == 1) {
+      const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const f32x4 s = tile[u].o[d] * inv;
+        *reinterpret_cast<uint2*>(a.out + sink_out_index(a, HD, t.b, r, kvh, d * 16 + 4 * g)) =
+            uint2{pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3])};
+      }
+    } else {
+      const int64_t row = ((int64_t)t.slot * a.nkv + kvh) * a.R + r;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(a.part_o + row * HD + d * 16 + 4 * g) = tile[u].o[d];
+      if (g == 0) *reinterpret_cast<float2*>(a.part_ml + row * 2) = float2{tile[u].m, l};
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------- splits joined
+// One workgroup per (row b, kv head, query row): 256 / (HD / 4) lanes over the splits, 4 dims each, then
+// over the lanes in LDS. Splits are added in a fixed order.
+template <int HD>
+__global__ __launch_bounds__(256) void attention_join_kernel(SinkArgs a) {
+  constexpr int C = HD / 4, S = 256 / C, U = 4;
+  __shared__ f32x4 acc_s[S][C];
+  __shared__ float2 ml_s[S];
+  const int r = blockIdx.x % a.R, bk = blockIdx.x / a.R, kvh = bk % a.nkv, b = bk / a.nkv;
+  const int ch = threadIdx.x % C, sl = threadIdx.x / C;
+  int first, live;
+  if (a.balanced) {
+    const int bps = balanced_blocks(a);
+    first = 0;
+    for (int x = 0; x < b; ++x) first += max(1, (key_plan(a, a.seq_lens[x], 0, a.W - 1).T + bps - 1) / bps);
+    live = max(1, (key_plan(a, a.seq_lens[b], 0, a.W - 1).T + bps - 1) / bps);
+  } else {
+    const int group = r / a.grows;
+    const int T = key_plan(a, a.seq_lens[b], group * a.grows / a.G, (min(a.R, (group + 1) * a.grows) - 1) / a.G).T;
+    const int bps = max(kMinSplitBlocks, round4((T + a.nsplit - 1) / a.nsplit));
+    first = b * a.nsplit;
+    live = max(1, (T + bps - 1) / bps);
+  }
+  if (live == 1) return;  // written whole
+  float M = -__builtin_inff(), L = 0.0f;
+  f32x4 acc = f32x4{0, 0, 0, 0};
+  for (int s0 = sl; s0 < live; s0 += S * U) {
+    float2 ml[U];
+    f32x4 o[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = min(s0 + u * S, live - 1);
+      const int64_t row = ((int64_t)(first + s) * a.nkv + kvh) * a.R + r;
+      ml[u] = *reinterpret_cast<const float2*>(a.part_ml + row * 2);
+      o[u] = *reinterpret_cast<const f32x4*>(a.part_o + row * HD + ch * 4);
+      if (s0 + u * S >= live) ml[u].x = -__builtin_inff();
+    }
+    float Mn = M;
+#pragma unroll
+    for (int u = 0; u < U; ++u) Mn = fmaxf(Mn, ml[u].x);
+    if (Mn == -__builtin_inff()) continue;
+    const float al = M == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(M - Mn);
+    L *= al;
+    acc *= al;
+    M = Mn;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (ml[u].x == -__builtin_inff()) continue;
+      const float w = __builtin_amdgcn_exp2f(ml[u].x - M);
+      L += w * ml[u].y;
+      acc += w * o[u];
+    }
+  }
+  acc_s[sl][ch] = acc;
+  if (ch == 0) ml_s[sl] = float2{M, L};
+  __syncthreads();
+  if (sl > 0) return;
+  float Mt = -__builtin_inff(), Lt = 0.0f;
+#pragma unroll
+  for (int s = 0; s < S; ++s) Mt = fmaxf(Mt, ml_s[s].x);
+  f32x4 tot = f32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    if (ml_s[s].x == -__builtin_inff()) continue;
+    const float w = __builtin_amdgcn_exp2f(ml_s[s].x - Mt);
+    Lt += w * ml_s[s].y;
+    tot += w * acc_s[s][ch];
+  }
+  const float inv = Lt != 0.0f ? 1.0f / Lt : 0.0f;
+  tot *= inv;
+  *reinterpret_cast<uint2*>(a.out + sink_out_index(a, HD, b, r, kvh, ch * 4)) =
+      uint2{pack_bf16x2(tot[0], tot[1]), pack_bf16x2(tot[2], tot[3])};
+}
+
+// ----------------------------------------------------------------------------- host
+// The launch of a pass, from its shape alone (a captured graph replays it for any lengths).
+struct SinkPlan {
+  bool tile;       // one tile of rows per workgroup, or blocks of rows
+  int waves, tpw;  // block kernel
+  int groups, grows, nsplit, balanced, slots;
+};
+static SinkPlan sink_plan(int B, int W, int nq, int nkv, int hd, int causal, int window, int sinks, int max_ctx) {
+  SinkPlan s = {};
+  const int64_t R = (int64_t)W * (nq / nkv);
+  s.tile = R <= 16;
+  if (!s.tile) {
+    const bool big = hd == 128 && R > 64;
+    s.waves = big ? 8 : 4;
+    s.tpw = big ? 2 : 1;
+  }
+  s.grows = s.tile ? 16 : s.waves * s.tpw * 16;
+  s.groups = (int)ceil_div(R, s.grows);
+  // blocks of 32 keys a pass may look at (the sliding window's rows, and its sinks)
+  int64_t span = max_ctx;
+  if (causal && window > 0) span = std::min<int64_t>(span, (int64_t)window + W + sinks + 96);
+  const int64_t most = std::max<int64_t>(1, ceil_div(ceil_div(span, 32) + 1, kMinSplitBlocks));
+  const int64_t tasks = (int64_t)B * nkv * s.groups, want = 512;
+  s.nsplit = (int)std::min<int64_t>(most, std::max<int64_t>(1, want / tasks));
+  s.balanced = s.groups == 1 && B <= kBalancedRows && B > 1 && s.nsplit > 1;
+  s.slots = s.balanced ? B * s.nsplit + B : B * s.nsplit;
+  return s;
+}
+static size_t sink_part_o_bytes(const SinkPlan& s, int64_t R, int nkv, int hd) {
+  return ((size_t)s.slots * nkv * R * hd * sizeof(float) + 255) & ~(size_t)255;
+}
+static size_t sink_ws(const SinkPlan& s, int64_t R, int nkv, int hd) {
+  return s.nsplit > 1 ? sink_part_o_bytes(s, R, nkv, hd) + (size_t)s.slots * nkv * R * 2 * sizeof(float) : 0;
+}
+
+template <int HD, int KVT>
+static void launch_sinks(const SinkArgs& a, const SinkPlan& s, hipStream_t st) {
+  const dim3 grid((unsigned)(s.slots * a.nkv), (unsigned)s.groups);
+  if (s.tile) {
+    hipLaunchKernelGGL((attention_tile_kernel<HD, KVT>), grid, dim3(256), 0, st, a);
+  } else if (s.waves == 8) {
+    if constexpr (HD == 128) hipLaunchKernelGGL((attention_block_kernel<HD, KVT, 8, 2>), grid, dim3(512), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((attention_block_kernel<HD, KVT, 4, 1>), grid, dim3(256), 0, st, a);
+  }
+  if (s.nsplit > 1)
+    hipLaunchKernelGGL((attention_join_kernel<HD>), dim3((unsigned)((int64_t)a.B * a.nkv * a.R)), dim3(256), 0, st, a);
+}
+
+}  // namespace dsk
+
+using namespace dsk;
+
+extern "C" size_t dsk_attention_sinks_ws_bytes(int B, int W, int nq, int nkv, int hd, int causal, int window, int sinks,
+                                               int max_ctx) {
+  if (B <= 0 || W <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || (hd != 128 && hd != 256) || max_ctx <= 0 || window < 0 || sinks < 0)
+    return 0;
+  return sink_ws(sink_plan(B, W, nq, nkv, hd, causal, window, sinks, max_ctx), (int64_t)W * (nq / nkv), nkv, hd);
+}
+
+extern "C" int dsk_attention_sinks(const uint16_t* q, int B, int W, int nq, int nkv, int hd, float scale, int causal,
+                                   int window, int sinks, float softcap, const int32_t* seq_lens, int max_ctx,
+                                   const int32_t* block_table, int max_pages, int page, int kv_dtype,
+                                   const void* k_pool, const void* v_pool, const uint32_t* k_sb, const uint32_t* v_sb,
+                                   uint16_t* out, int out_packed, void* workspace, size_t ws_bytes,
+                                   dsk_stream_t stream) {
+  const char* who = "dsk_attention_sinks";
+  DSK_REQUIRE(q && seq_lens && block_table && k_pool && v_pool && out, "%s: null pointer", who);
+  DSK_REQUIRE(hd == 128 || hd == 256, "%s: head_dim %d not supported (128, 256)", who, hd);
+  DSK_REQUIRE(B > 0 && W > 0 && nq > 0 && nkv > 0 && nq % nkv == 0, "%s: bad shape", who);
+  DSK_REQUIRE(scale > 0.0f && softcap >= 0.0f, "%s: scale must be positive, softcap not negative", who);
+  DSK_REQUIRE(window >= 0 && sinks >= 0 && window < 0x20000000 && sinks < 0x20000000, "%s: window %d, sinks %d", who, window, sinks);
+  DSK_REQUIRE(kv_dtype == DSK_KV_BF16 || kv_dtype == DSK_KV_U8 || kv_dtype == DSK_KV_U4, "%s: kv_dtype %d", who, kv_dtype);
+  DSK_REQUIRE(kv_dtype == DSK_KV_BF16 || (k_sb && v_sb), "%s: quantised KV needs scale/bias buffers", who);
+  DSK_REQUIRE(page > 0 && page % kKv4Block == 0 && max_pages > 0, "%s: pages are multiples of %d tokens (got %d)", who, kKv4Block,
+              page);
+  DSK_REQUIRE(max_ctx >= W && (int64_t)max_pages * page >= max_ctx && (int64_t)max_pages * page < 0x20000000,
+              "%s: max_ctx %d beyond block table", who, max_ctx);
+  DSK_REQUIRE((((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out) & 15) == 0,
+              "%s: q, pools and out must be 16-byte aligned", who);
+  DSK_REQUIRE(!out_packed || (B * W <= 64 && (nq * hd) % 64 == 0), "%s: packed output needs B*W <= 64", who);
+  const int64_t R = (int64_t)W * (nq / nkv);
+  const SinkPlan s = sink_plan(B, W, nq, nkv, hd, causal, window, sinks, max_ctx);
+  DSK_REQUIRE(R <= 0x7fffffff && s.groups <= 65535 && (int64_t)s.slots * nkv <= 0x7fffffff && (int64_t)B * nkv * R <= 0x7fffffff,
+              "%s: %lld query rows per kv head", who, (long long)R);
+  const size_t need = sink_ws(s, R, nkv, hd);
+  if (need && (!workspace || ws_bytes < need)) {
+    set_error("%s: workspace %zu < %zu", who, ws_bytes, need);
+    return DSK_ENOWS;
+  }
+  DSK_REQUIRE(((uintptr_t)workspace & 15) == 0 || need == 0, "%s: workspace must be 16-byte aligned", who);
+  SinkArgs a = {q, B, W, nq, nkv, nq / nkv, (int)R, scale, softcap, causal ? 1 : 0, window, sinks, seq_lens, block_table,
+                max_pages, page, k_pool, v_pool, k_sb, v_sb, out, out_packed ? 1 : 0, s.groups, s.grows, s.slots, s.nsplit,
+                s.balanced, reinterpret_cast<float*>(workspace),
+                reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + sink_part_o_bytes(s, R, nkv, hd))};
+#define DSK_SINKS(HDV)                                                                                \
+  if (kv_dtype == DSK_KV_BF16) launch_sinks<HDV, DSK_KV_BF16>(a, s, as_stream(stream));               \
+  else if (kv_dtype == DSK_KV_U8) launch_sinks<HDV, DSK_KV_U8>(a, s, as_stream(stream));              \
+  else launch_sinks<HDV, DSK_KV_U4>(a, s, as_stream(stream))
+  if (hd == 128) {
+    DSK_SINKS(128);
+  } else {
+    DSK_SINKS(256);
+  }
+#undef DSK_SINKS
+  DSK_LAUNCH_CHECK(who);
+  return DSK_OK;
+}

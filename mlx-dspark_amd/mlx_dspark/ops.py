@@ -519,12 +519,30 @@ def kv_read(first, n, nkv, hd, block_table, page, kv_dtype, k_pool, v_pool, k_sb
 
 
 def attention(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table, page, kv_dtype, k_pool,
-              v_pool, k_sb=None, v_sb=None, *, causal=True, window=0, softcap=0.0, out=None, packed=False):
-    """Returns bf16 [B*W, nq*hd], or a Packed [B*W, nq*hd] (the o-projection's x) when packed."""
+              v_pool, k_sb=None, v_sb=None, *, causal=True, window=0, softcap=0.0, out=None, packed=False, sinks=0):
+    """Returns bf16 [B*W, nq*hd], or a Packed [B*W, nq*hd] (the o-projection's x) when packed. sinks: the
+    context's first tokens that stay visible beside a sliding window (causal). 4-bit caches and sinks run
+    dsk_attention_sinks, which takes any W."""
     if out is None:
         out = Packed.empty(B * W, nq * hd, q.device) if packed else torch.empty(
             (B * W, nq * hd), dtype=torch.bfloat16, device=q.device)
     odata = out.data if isinstance(out, Packed) else out
+    if sinks or kv_dtype == DSK_KV_U4:
+        _on_device(q)
+        if q.dtype != torch.bfloat16 or not q.is_contiguous() or q.numel() != B * W * nq * hd:
+            raise ValueError(f"attention: q must be contiguous bf16 [{B * W}, {nq * hd}]")
+        if odata.dtype != torch.bfloat16 or not odata.is_contiguous() or (
+                not isinstance(out, Packed) and odata.numel() != B * W * nq * hd):
+            raise ValueError(f"attention: out must be contiguous bf16 [{B * W}, {nq * hd}]")
+        need = _hip.lib.dsk_attention_sinks_ws_bytes(B, W, nq, nkv, hd, int(bool(causal)), int(window), int(sinks),
+                                                     int(max_ctx))
+        # per call: passes on two streams, or of two captured graphs, may overlap
+        buf = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        call("dsk_attention_sinks", ptr(q), B, W, nq, nkv, hd, float(scale), int(bool(causal)), int(window),
+             int(sinks), float(softcap), ptr(seq_lens), int(max_ctx), ptr(block_table), block_table.shape[1], page,
+             kv_dtype, ptr(k_pool), ptr(v_pool), ptr(k_sb), ptr(v_sb), ptr(odata), int(isinstance(out, Packed)),
+             ptr(buf), need, stream_ptr())
+        return out
     ws = Workspace.get(q.device)
     need = _hip.lib.dsk_attn_ws_bytes(B, W, nq, hd, max_ctx)
     buf = ws.reserve("attn", need)
@@ -562,13 +580,14 @@ def attention_rows_split(L: int, nq: int, nkv: int, hd: int, cached: int, max_ct
 
 
 def attention_rows(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table, page, kv_dtype, k_pool, v_pool,
-                   k_sb=None, v_sb=None, *, causal=True, window=0):
+                   k_sb=None, v_sb=None, *, causal=True, window=0, sinks=0):
     """attention of a prompt's many rows, bf16 [B*W, nq*hd], with the verify kernels' float32
     probabilities (dsk_attention_rows; dsk_attention where its shapes end, with scratch for every row and
-    key split: by attention_rows_takes a caller can give that one fewer rows at a time)."""
-    if not attention_rows_takes(hd, block_table.shape[1]):
+    key split: by attention_rows_takes a caller can give that one fewer rows at a time). 4-bit caches and
+    sinks: as attention."""
+    if sinks or kv_dtype == DSK_KV_U4 or not attention_rows_takes(hd, block_table.shape[1]):
         return attention(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table, page, kv_dtype, k_pool, v_pool,
-                         k_sb, v_sb, causal=causal, window=window)
+                         k_sb, v_sb, causal=causal, window=window, sinks=sinks)
     out = torch.empty((B * W, nq * hd), dtype=torch.bfloat16, device=q.device)
     call("dsk_attention_rows", ptr(q), B, W, nq, nkv, hd, float(scale), int(bool(causal)), int(window), ptr(seq_lens),
          ptr(block_table), block_table.shape[1], page, kv_dtype, ptr(k_pool), ptr(v_pool), ptr(k_sb), ptr(v_sb),

@@ -50,3 +50,35 @@ def test_cache_refuses():
             PagedKVCache(1, 1, 2, 128, 64, device="cpu", **kw)
     with pytest.raises(ValueError):
         PagedKVCache(1, 1, 2, 512, 64, device="cpu", kv_bits=4)
+
+
+def _attend(**kw):
+    from mlx_dspark import _hip
+    a = dict(q=P, B=1, W=1, nq=4, nkv=2, hd=128, scale=0.1, causal=1, window=0, sinks=0, cap=0.0, sl=P, max_ctx=100,
+             table=P, max_pages=2, page=64, kv=2, k=P, v=P, ks=P, vs=P, out=P, packed=0, ws=None, wsb=0, st=None)
+    a.update(kw)
+    return _hip.lib.dsk_attention_sinks(*a.values()), _hip.lib.dsk_last_error().decode()
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(q=None), "null"), (dict(hd=512), "head_dim"), (dict(nq=3), "shape"), (dict(W=0), "shape"),
+    (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(cap=-1.0), "softcap"), (dict(window=-1), "window"),
+    (dict(sinks=-1), "sinks"), (dict(kv=3), "kv_dtype"), (dict(ks=None), "scale/bias"), (dict(kv=0, page=48), "multiples of 32"),
+    (dict(page=16), "multiples of 32"), (dict(max_ctx=129), "max_ctx"), (dict(W=2, max_ctx=1), "max_ctx"),
+    (dict(out=ctypes.c_void_p((1 << 20) + 8)), "aligned"), (dict(W=65, packed=1), "packed"),
+    (dict(max_pages=1 << 24), "block table"),
+])
+def test_attention_refuses(kw, word):
+    rc, msg = _attend(**kw)
+    assert rc == -1 and word in msg, msg
+
+
+def test_attention_workspace_too_small():
+    from mlx_dspark import _hip
+
+    need = _hip.lib.dsk_attention_sinks_ws_bytes(1, 1, 4, 2, 128, 1, 0, 0, 4096)
+    assert need > 0
+    for ws, n in ((None, 0), (P, need - 1)):
+        rc, msg = _attend(max_ctx=4096, max_pages=64, ws=ws, wsb=n)
+        assert rc == -4 and "workspace" in msg
+    assert _hip.lib.dsk_attention_sinks_ws_bytes(1, 1, 4, 2, 64, 1, 0, 0, 4096) == 0
