@@ -190,26 +190,39 @@ struct Tile {
     hi = u32x4{h[0], h[1], h[2], h[3]};
     lo = u32x4{w[0], w[1], w[2], w[3]};
   }
-  // O^T += V^T . P^T where a key that some query does not see holds an infinity or a NaN: key by key, each
-  // kept out of the queries that do not see it
-  template <class VF>
-  __device__ __forceinline__ void add_guarded(const Sight& see, int base, int lane, u32x4 hi, u32x4 lo, VF vf) {
+  // The infinities and NaN of a block whose keys not every query sees: the matrix products took it without
+  // them (finite_only), and each is added here to the queries that see its key. raw(d, k, g, r): the bf16
+  // value of key k, dim 16 d + 4 g + r. Rare, and written to cost the common path no registers.
+  template <class Raw>
+  __device__ __forceinline__ void add_nonfinite(const Sight& see, int base, int lane, u32x4 hi, u32x4 lo, Raw raw) {
 #pragma unroll 1
     for (int k = 0; k < 32; ++k) {
-      const int e = (k / 16) * 4 + k % 4;
-      const bool mine = (lane >> 4) == (k % 16) / 4, vis = see.sees(base + k);
-      u32x4 keep;
+      const int e = (k / 16) * 4 + k % 4, from = (lane & 15) + 16 * ((k % 16) / 4);
+      const uint32_t h = e < 4 ? (e < 2 ? hi[0] : hi[1]) : (e < 6 ? hi[2] : hi[3]);
+      const uint32_t w = e < 4 ? (e < 2 ? lo[0] : lo[1]) : (e < 6 ? lo[2] : lo[3]);
+      const int sh = e & 1 ? 0 : 16;
+      float p = bits_f32((h << sh) & 0xffff0000u) + bits_f32((w << sh) & 0xffff0000u);
+      p = __shfl(p, from, 64);
+      const bool vis = see.sees(base + k);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) keep[w] = mine && w == e / 2 ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
+      for (int d = 0; d < HD / 16; ++d)
 #pragma unroll
-      for (int d = 0; d < HD / 16; ++d) {
-        const u32x4 v = vf(d) & keep;
-        const f32x4 t = mfma16(v, lo, mfma16(v, hi, o[d]));
-        o[d] = vis ? t : o[d];
-      }
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t v = raw(d, k, lane >> 4, r);
+          const bool add = bool((int)((v & 0x7f80u) == 0x7f80u) & (int)vis);
+          o[d][r] = add ? fmaf(p, bits_f32(v << 16), o[d][r]) : o[d][r];
+        }
     }
   }
 };
+__device__ __forceinline__ u32x4 finite_only(u32x4 x) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const uint32_t l = (x[w] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu, h = (x[w] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u;
+    x[w] &= l | h;
+  }
+  return x;
+}
 
 // masks of a 32-key block's (or two blocks') scores: lane holds keys base + 16 t + 4 g + r
 template <int NKT>
@@ -474,14 +487,23 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 4))) voi
       }
       guarded = __any(bad);
     }
-    if (guarded) {
-      tile.add_guarded(see, base, lane, hi, lo, operand);
-    } else {
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const u32x4 x = operand(d);
-        tile.o[d] = mfma16(x, lo, mfma16(x, hi, tile.o[d]));
-      }
+    for (int d = 0; d < DT; ++d) {
+      u32x4 x = operand(d);
+      if (guarded) x = finite_only(x);
+      tile.o[d] = mfma16(x, lo, mfma16(x, hi, tile.o[d]));
+    }
+    if (guarded) {
+      tile.add_nonfinite(see, base, lane, hi, lo, [&](int d, int k, int gg, int rr) -> uint32_t {
+        const int e = (k / 16) * 4 + k % 4, at = 4 * gg + rr + 16 * ((k % 16) / 4);  // the lane that holds it
+        if constexpr (kRows) {
+          return *reinterpret_cast<const uint16_t*>(vlds + d * kVTile + (at >> 4) * kVGroup + (at & 15) * 16 + 2 * e);
+        } else {
+          const u32x4& x = vf[kRows ? 0 : d];
+          const uint32_t w = __shfl(e < 4 ? (e < 2 ? x[0] : x[1]) : (e < 6 ? x[2] : x[3]), at, 64);
+          return e & 1 ? w >> 16 : w & 0xffffu;
+        }
+      });
     }
     if constexpr (kRows) asm volatile("" ::: "memory");
   }
@@ -689,27 +711,32 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
     for (int x = 0; x < NB; ++x) {
       const uint8_t* vb8 = &vbuf[buf][x * DT * kVTile];
-      auto operand = [&](int d) { return v_operand(vb8, d, lane); };
+      bool guarded = false;
       if (!open) {
         bool bad = false;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          const u32x4 w = operand(d);
+          const u32x4 w = v_operand(vb8, d, lane);
           bad |= nonfinite2(w[0]) || nonfinite2(w[1]) || nonfinite2(w[2]) || nonfinite2(w[3]);
         }
-        if (__any(bad)) {
-#pragma unroll
-          for (int u = 0; u < TPW; ++u) tile[u].add_guarded(see[u], base[x], lane, hi[u][x], lo[u][x], operand);
-          continue;
-        }
+        guarded = __any(bad);
       }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        const u32x4 w = operand(d);
+        u32x4 w = v_operand(vb8, d, lane);
+        if (guarded) w = finite_only(w);
 #pragma unroll
         for (int u = 0; u < TPW; ++u) tile[u].o[d] = mfma16(w, hi[u][x], tile[u].o[d]);
 #pragma unroll
         for (int u = 0; u < TPW; ++u) tile[u].o[d] = mfma16(w, lo[u][x], tile[u].o[d]);
+      }
+      if (guarded) {
+#pragma unroll
+        for (int u = 0; u < TPW; ++u)
+          tile[u].add_nonfinite(see[u], base[x], lane, hi[u][x], lo[u][x], [&](int d, int k, int gg, int rr) -> uint32_t {
+            return *reinterpret_cast<const uint16_t*>(vb8 + d * kVTile + ((k % 16) / 4) * kVGroup + (4 * gg + rr) * 16 +
+                                                      2 * ((k / 16) * 4 + k % 4));
+          });
       }
     }
   };
