@@ -11,11 +11,23 @@
 // The maximum moves only when a score passes it by 2^8: below that the exponentials stay in float32's
 // range and nothing is lost, and a block costs one vote instead of two lane exchanges and a rescale.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "kv4.h"
 
 namespace dsk {
+
+// x / d for 0 <= x < 2^31 by a multiplication (d is the same for a whole launch): a division costs a wave
+// some 30 instructions, a dozen of them stood before a split's first load.
+struct FastDiv {
+  uint32_t d, m, s;
+  __host__ explicit FastDiv(uint32_t v = 1) : d(v), s(0) {
+    while ((1ull << s) < v) ++s;
+    m = (uint32_t)(((1ull << 32) * ((1ull << s) - v)) / v + 1);
+  }
+  __device__ __forceinline__ int quot(int x) const { return (int)((__umulhi((uint32_t)x, m) + (uint32_t)x) >> s); }
+};
 
 struct SinkArgs {
   const uint16_t* q;  // [B*W][nq*HD]
@@ -31,16 +43,16 @@ struct SinkArgs {
   int out_packed;
   int groups;    // row groups of a (row b, kv head), one workgroup each per split
   int grows;     // rows per group
-  int slots;     // splits on the grid per kv head: balanced over the rows' lengths (groups == 1), or
-                 // nsplit for each row and group
+  int slots;     // splits on the grid per kv head: placed by the rows' lengths (balanced), or nsplit for each row
   int nsplit, balanced;
+  int unit;        // splits are multiples of this many 32-key blocks (a power of two)
   float* part_o;   // [slot][kv head][R][HD] unnormalised outputs
   float* part_ml;  // [slot][kv head][R][2] running maximum (of scores times c2) and sum
+  FastDiv by_page, by_G, by_nkv, by_nsplit;
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kMaxSlack = 8.0f;   // how far (log2) a score may pass the running maximum
-constexpr int kMinSplitBlocks = 4;  // 32-key blocks per split at least: one per wave
 constexpr int kBalancedRows = 64;   // rows whose lengths a workgroup reads to place its split
 
 // The 32-key blocks that query tokens i0 .. i1 of row b look at.
@@ -62,7 +74,6 @@ __device__ __forceinline__ KeyPlan key_plan(const SinkArgs& a, int len, int i0, 
   p.T = p.nA + (p.j_end - p.beg + 31) / 32;
   return p;
 }
-__device__ __forceinline__ int round4(int x) { return (x + 3) & ~3; }
 
 // Which split a workgroup runs: the row b, its slot of the partial buffers, its blocks [v0, v1) and the
 // number of splits that the row (and group) has. Balanced: blocks per split from the rows' summed lengths, so that rows
@@ -74,7 +85,11 @@ struct SplitTask {
 __device__ __forceinline__ int balanced_blocks(const SinkArgs& a) {
   int total = 0;
   for (int b = 0; b < a.B; ++b) total += key_plan(a, a.seq_lens[b], 0, a.W - 1).T;
-  return max(kMinSplitBlocks, round4((total + a.slots - a.B - 1) / (a.slots - a.B)));
+  // sum of ceil(T / bps) <= (slots - B) + B
+  return max(a.unit, ((total + a.slots - a.B - 1) / (a.slots - a.B) + a.unit - 1) & -a.unit);
+}
+__device__ __forceinline__ int even_blocks(const SinkArgs& a, int T) {
+  return max(a.unit, (a.by_nsplit.quot(T + a.nsplit - 1) + a.unit - 1) & -a.unit);
 }
 __device__ __forceinline__ SplitTask split_task(const SinkArgs& a, int slot, int group) {
   SplitTask t;
@@ -98,10 +113,10 @@ __device__ __forceinline__ SplitTask split_task(const SinkArgs& a, int slot, int
     }
     return t;
   }
-  t.b = slot / a.nsplit;
-  t.p = key_plan(a, a.seq_lens[t.b], group * a.grows / a.G, (min(a.R, (group + 1) * a.grows) - 1) / a.G);
-  const int bps = max(kMinSplitBlocks, round4((t.p.T + a.nsplit - 1) / a.nsplit));
-  const int s = slot % a.nsplit, live = max(1, (t.p.T + bps - 1) / bps);
+  t.b = a.by_nsplit.quot(slot);
+  t.p = key_plan(a, a.seq_lens[t.b], a.by_G.quot(group * a.grows), a.by_G.quot(min(a.R, (group + 1) * a.grows) - 1));
+  const int bps = even_blocks(a, t.p.T);
+  const int s = slot - t.b * a.nsplit, live = max(1, (t.p.T + bps - 1) / bps);
   if (s < live) t.live = live;
   t.v0 = s * bps;
   t.v1 = min(t.p.T, t.v0 + bps);
@@ -140,8 +155,17 @@ __device__ __forceinline__ bool nonfinite2(uint32_t w) {
   return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
 __device__ __forceinline__ int64_t sink_out_index(const SinkArgs& a, int HD, int b, int r, int kvh, int d) {
-  const int64_t m = (int64_t)b * a.W + r / a.G, k = (int64_t)(kvh * a.G + r % a.G) * HD + d;
+  const int i = a.by_G.quot(r);
+  const int64_t m = (int64_t)b * a.W + i, k = (int64_t)(kvh * a.G + r - i * a.G) * HD + d;
   return a.out_packed ? apack_index(m, k, (int64_t)a.nq * HD / 64) : m * a.nq * HD + k;
+}
+
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void static_for(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    static_for<N, I + 1>(f);
+  }
 }
 
 // The running state of one tile of 16 queries over the keys seen so far.
@@ -190,10 +214,20 @@ struct Tile {
     hi = u32x4{h[0], h[1], h[2], h[3]};
     lo = u32x4{w[0], w[1], w[2], w[3]};
   }
-  // The infinities and NaN of a block whose keys not every query sees: the matrix products took it without
-  // them (finite_only), and each is added here to the queries that see its key. raw(d, k, g, r): the bf16
-  // value of key k, dim 16 d + 4 g + r. Rare, and written to cost the common path no registers.
-  template <class Raw>
+  // O^T += V^T . P^T for d tiles D .. D + 3 and a block's 32 keys. The first terms of the four, then the
+  // second ones: four independent products between two on the same accumulator.
+  template <int D>
+  __device__ __forceinline__ void add4(const u32x4 (&v)[4], u32x4 hi, u32x4 lo) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[D + d] = mfma16(v[d], hi, o[D + d]);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[D + d] = mfma16(v[d], lo, o[D + d]);
+  }
+  // The infinities and NaN of those operands, where not every query sees every key: the products take the
+  // operands without them (finite_only), and each is added here to the queries that see its key.
+  // raw(d, k, g, r): the bf16 value of key k, dim 16 (D + d) + 4 g + r. Rare, and written to cost the common
+  // path no registers.
+  template <int D, class Raw>
   __device__ __forceinline__ void add_nonfinite(const Sight& see, int base, int lane, u32x4 hi, u32x4 lo, Raw raw) {
 #pragma unroll 1
     for (int k = 0; k < 32; ++k) {
@@ -205,16 +239,24 @@ struct Tile {
       p = __shfl(p, from, 64);
       const bool vis = see.sees(base + k);
 #pragma unroll
-      for (int d = 0; d < HD / 16; ++d)
+      for (int d = 0; d < 4; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const uint32_t v = raw(d, k, lane >> 4, r);
           const bool add = bool((int)((v & 0x7f80u) == 0x7f80u) & (int)vis);
-          o[d][r] = add ? fmaf(p, bits_f32(v << 16), o[d][r]) : o[d][r];
+          o[D + d][r] = add ? fmaf(p, bits_f32(v << 16), o[D + d][r]) : o[D + d][r];
         }
     }
   }
 };
+__device__ __forceinline__ bool any_nonfinite(const u32x4 (&v)[4]) {
+  bool bad = false;
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) bad |= nonfinite2(v[d][w]);
+  return __any(bad);
+}
 __device__ __forceinline__ u32x4 finite_only(u32x4 x) {
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
@@ -252,11 +294,16 @@ __device__ __forceinline__ u32x4 kv8_row8(uint2 r, uint32_t z) {
 // ----------------------------------------------------------------------------- K and V of a block
 // One wave's loads of a 32-key block, kept raw until they are used (so the next block's are in flight
 // meanwhile), and the operands they become.
+// Every member is one load: parts of a wider load held in separate variables would be copied (and so
+// waited for) where the loop comes round.
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 // K: u32x4 per 16-key tile and 32-dim step (A operand of the score product).
 template <int HD, int KVT>
 struct KRaw {
-  u32x4 q[2][KVT == DSK_KV_BF16 ? HD / 32 : (KVT == DSK_KV_U8 ? HD / 64 : HD / 128)];
-  uint32_t sb[2][KVT == DSK_KV_BF16 ? 1 : HD / 64];
+  static constexpr bool kBytes = KVT == DSK_KV_U8;
+  u32x4 q[2][KVT == DSK_KV_BF16 ? HD / 32 : (kBytes ? 1 : HD / 128)];
+  u32x2 h[2][kBytes ? HD / 32 : 1];  // 8-bit: 8 dims of each step
+  u32x2 sb[2][KVT == DSK_KV_BF16 ? 1 : HD / 128];
   // tok: pool token of the block's first key
   __device__ __forceinline__ void load(const SinkArgs& a, uint32_t tok, int lane) {
     const int n = lane & 15, g = lane >> 4;
@@ -267,13 +314,10 @@ struct KRaw {
         const uint16_t* src = reinterpret_cast<const uint16_t*>(a.k_pool) + row * HD + 8 * g;
 #pragma unroll
         for (int s = 0; s < HD / 32; ++s) q[t][s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
-      } else if constexpr (KVT == DSK_KV_U8) {
+      } else if constexpr (kBytes) {
         const uint8_t* src = reinterpret_cast<const uint8_t*>(a.k_pool) + row * HD + 8 * g;
 #pragma unroll
-        for (int s = 0; s < HD / 64; ++s) {
-          const uint2 x = *reinterpret_cast<const uint2*>(src + 64 * s), y = *reinterpret_cast<const uint2*>(src + 64 * s + 32);
-          q[t][s] = u32x4{x.x, x.y, y.x, y.y};
-        }
+        for (int s = 0; s < HD / 32; ++s) h[t][s] = *reinterpret_cast<const u32x2*>(src + 32 * s);
       } else {
         const uint8_t* src = reinterpret_cast<const uint8_t*>(a.k_pool) + row * (HD / 2) + 16 * g;
 #pragma unroll
@@ -281,15 +325,14 @@ struct KRaw {
       }
       if constexpr (KVT != DSK_KV_BF16) {
 #pragma unroll
-        for (int c = 0; c < HD / 64; ++c) sb[t][c] = a.k_sb[row * (HD / 64) + c];
+        for (int c = 0; c < HD / 128; ++c) sb[t][c] = *reinterpret_cast<const u32x2*>(a.k_sb + row * (HD / 64) + 2 * c);
       }
     }
   }
   __device__ __forceinline__ u32x4 operand(int t, int s) const {
     if constexpr (KVT == DSK_KV_BF16) return q[t][s];
-    else if constexpr (KVT == DSK_KV_U8)
-      return kv8_row8(s & 1 ? uint2{q[t][s / 2][2], q[t][s / 2][3]} : uint2{q[t][s / 2][0], q[t][s / 2][1]}, sb[t][s / 2]);
-    else return kv4_row8(q[t][s / 4][s % 4], kv4_scale(sb[t][s / 2]));
+    else if constexpr (kBytes) return kv8_row8(uint2{h[t][s][0], h[t][s][1]}, sb[t][s / 4][(s / 2) & 1]);
+    else return kv4_row8(q[t][s / 4][s % 4], kv4_scale(sb[t][s / 4][(s / 2) & 1]));
   }
 };
 
@@ -323,16 +366,68 @@ struct V4Raw {
     }
   }
   __device__ __forceinline__ void drop_dead(const SinkArgs& a, const KeyPlan& p, int base, int lane) {
+    asm volatile("" : "+s"(base));  // keeps the tests inside the caller's branch
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       sb[e] = key_dead(a, p, base + 16 * (e / 4) + 4 * (lane >> 4) + e % 4) ? 0u : sb[e];
   }
 };
 
+// All of a block's 4-bit V: chunk c's 16 bytes and, per 16-key tile, the words of 4 keys
+template <int HD>
+struct V4Block {
+  u32x4 q[HD / 64];
+  u32x4 sb[2][HD / 64];  // word (r, c) of tile u: element r * (HD / 64) + c of sb[u]
+  __device__ __forceinline__ void load(const SinkArgs& a, uint32_t tok, int lane) {
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(a.v_pool) + (int64_t)tok * (HD / 2) + lane * 16;
+    const uint32_t* w = a.v_sb + ((int64_t)tok + 4 * (lane >> 4)) * (HD / 64);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int x = 0; x < HD / 64; ++x) sb[u][x] = *reinterpret_cast<const u32x4*>(w + 16 * u * (HD / 64) + 4 * x);
+#pragma unroll
+    for (int c = 0; c < HD / 64; ++c) q[c] = *reinterpret_cast<const u32x4*>(src + c * 1024);
+  }
+  __device__ __forceinline__ void pin() {  // as VRowsRaw::pin
+#pragma unroll
+    for (int x = 0; x < HD / 64; ++x) asm volatile("" : "+v"(q[x]), "+v"(sb[0][x]), "+v"(sb[1][x]));
+  }
+  __device__ __forceinline__ void drop_dead(const SinkArgs& a, const KeyPlan& p, int base, int lane) {
+    asm volatile("" : "+s"(base));  // keeps the tests inside the caller's branch
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t keep = key_dead(a, p, base + 16 * u + 4 * (lane >> 4) + r) ? 0u : ~0u;
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c) sb[u][(r * (HD / 64) + c) / 4][(r * (HD / 64) + c) % 4] &= keep;
+      }
+  }
+  // d tiles 4 c + 2 p + h
+  __device__ __forceinline__ void operands(int c, u32x4 (&v)[4]) const {
+    Kv4Scale z[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int x = (e % 4) * (HD / 64) + c;
+      z[e] = kv4_scale(sb[e / 4][x / 4][x % 4]);
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      uint32_t lo[2][2], hi[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) kv4_col4(q[c][2 * p + u], z + 4 * u, lo[u], hi[u]);
+      v[2 * p] = u32x4{lo[0][0], lo[0][1], lo[1][0], lo[1][1]};
+      v[2 * p + 1] = u32x4{hi[0][0], hi[0][1], hi[1][0], hi[1][1]};
+    }
+  }
+};
+
 // row-major V (bf16, 8-bit): 4 keys x 8 dims, transposed on their way into the operand order in LDS
 template <int HD, int KVT>
 struct VRowsRaw {
-  u32x4 q[4];
+  static constexpr bool kBytes = KVT == DSK_KV_U8;
+  u32x4 q[kBytes ? 1 : 4];
+  u32x2 h[kBytes ? 4 : 1];
   uint32_t sb[4];
   // quad: keys 4 quad .. + 3 of the block, ch: dims 8 ch .. + 7
   __device__ __forceinline__ void load(const SinkArgs& a, uint32_t tok, int quad, int ch) {
@@ -342,10 +437,19 @@ struct VRowsRaw {
       if constexpr (KVT == DSK_KV_BF16) {
         q[r] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(a.v_pool) + row * HD + 8 * ch);
       } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(a.v_pool) + row * HD + 8 * ch);
-        q[r] = u32x4{x.x, x.y, 0, 0};
+        h[r] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint8_t*>(a.v_pool) + row * HD + 8 * ch);
         sb[r] = a.v_sb[row * (HD / 64) + ch / 8];
       }
+    }
+  }
+  // not used before this point: the scheduler would otherwise turn V into operands (and wait for it) while
+  // the scores are still on their way
+  __device__ __forceinline__ void pin() {
+    if constexpr (kBytes) {
+      asm volatile("" : "+v"(h[0]), "+v"(h[1]), "+v"(h[2]), "+v"(h[3]));
+      asm volatile("" : "+v"(sb[0]), "+v"(sb[1]), "+v"(sb[2]), "+v"(sb[3]));
+    } else {
+      asm volatile("" : "+v"(q[0]), "+v"(q[1]), "+v"(q[2]), "+v"(q[3]));
     }
   }
   // base: the block's first key; dst: the block's operands in LDS
@@ -354,8 +458,8 @@ struct VRowsRaw {
     u32x4 w[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      if constexpr (KVT == DSK_KV_BF16) w[r] = q[r];
-      else w[r] = kv8_row8(uint2{q[r][0], q[r][1]}, sb[r]);
+      if constexpr (kBytes) w[r] = kv8_row8(uint2{h[r][0], h[r][1]}, sb[r]);
+      else w[r] = q[r];
       const uint32_t keep = check && key_dead(a, p, base + 4 * quad + r) ? 0u : ~0u;
       w[r] &= u32x4{keep, keep, keep, keep};
     }
@@ -377,135 +481,160 @@ __device__ __forceinline__ u32x4 v_operand(const uint8_t* blk, int d, int lane) 
 // One tile of 16 query rows per workgroup; its split's blocks go round its four waves, each with a running
 // state of its own, merged in LDS at the end. No barrier before that: a wave turns its own loads into its
 // own operands (4-bit V lies in operand order; row-major V is transposed through the wave's LDS).
-// Page ids of 64 blocks are loaded at once, one per lane.
+// Page ids of 64 steps' blocks are loaded at once, one per lane.
+//
+// Bound by the instructions that turn codes into operands (17 for 8 codes: at 2 waves per SIMD a
+// v_fma_mix_f32 or v_cvt_pk takes 2.1 ns of a SIMD, a v_and or v_fma 1.3), not by memory. A step is NB
+// blocks: with one, the chain from scores to probabilities has too few independent instructions to hide
+// its latencies behind.
+template <int HD> constexpr int kTileBlocks = HD == 128 ? 2 : 1;  // registers
+
 template <int HD, int KVT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 4))) void attention_tile_kernel(SinkArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 2 : 1, 2))) void attention_tile_kernel(SinkArgs a) {
   constexpr int KS = HD / 32, DT = HD / 16, NI = HD / 128 * 2;  // NI: (quad, chunk) items per lane
+  constexpr int NB = kTileBlocks<HD>;
   constexpr bool kRows = KVT != DSK_KV_U4;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kRows && 4 * DT * kVTile > 4 * DT * 1024 ? 4 * DT * kVTile : 4 * DT * 1024];
   __shared__ float2 wml[4][16];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.x % a.nkv, group = blockIdx.y;
-  const SplitTask t = split_task(a, blockIdx.x / a.nkv, group);
+  const int slot = a.by_nkv.quot(blockIdx.x), kvh = blockIdx.x - slot * a.nkv, group = blockIdx.y;
+  const SplitTask t = split_task(a, slot, group);
   if (t.live == 0) return;
   const KeyPlan& p = t.p;
   const int r0 = group * a.grows, r = r0 + n, rc = min(r, a.R - 1);
-  const int pos = p.off + rc / a.G, pos_lo = p.off + r0 / a.G, pos_hi = p.off + (min(r0 + 16, a.R) - 1) / a.G;
+  const int ri = a.by_G.quot(rc);
+  const int pos = p.off + ri, pos_lo = p.off + a.by_G.quot(r0), pos_hi = p.off + a.by_G.quot(min(r0 + 16, a.R) - 1);
   const float c2 = (a.softcap > 0.0f ? 1.0f : a.scale) * kLog2e;
   const Sight see = sight(a, p, pos);
 
-  const int nblk = t.v1 > t.v0 + wv ? (t.v1 - t.v0 - wv + 3) / 4 : 0;  // this wave's blocks v0 + wv + 4 i
-  uint32_t toks = 0;  // lane l: pool token of block i = (i0 & ~63) + l
+  // this wave's steps: blocks v0 + NB (wv + 4 i) .. + NB - 1
+  const int left = t.v1 - t.v0 - NB * wv, nstep = left > 0 ? (left + 4 * NB - 1) / (4 * NB) : 0;
+  uint32_t toks[NB];  // lane l: pool tokens of the blocks of step (i & ~63) + l (past the split: its last block)
   auto find_tokens = [&](int i) {
-    const int base = p.base(min(t.v0 + wv + 4 * (i + lane), t.v1 - 1));
-    const int pg = a.block_table[(int64_t)t.b * a.max_pages + base / a.page];
-    toks = ((uint32_t)pg * a.nkv + kvh) * a.page + base % a.page;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int base = p.base(min(t.v0 + NB * (wv + 4 * (i + lane)) + b, t.v1 - 1));
+      const int lp = a.by_page.quot(base), pg = a.block_table[(int64_t)t.b * a.max_pages + lp];
+      toks[b] = ((uint32_t)pg * a.nkv + kvh) * a.page + (base - lp * a.page);
+    }
   };
-  auto token = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane(toks, i & 63); };
+  auto token = [&](int i, int b) { return (uint32_t)__builtin_amdgcn_readlane(toks[b], i & 63); };
 
-  KRaw<HD, KVT> k;
-  V4Raw<HD> v4[kRows ? 1 : HD / 64];
-  VRowsRaw<HD, KVT> vr[kRows ? NI : 1];
-  auto load_v = [&](uint32_t tok) {
+  KRaw<HD, KVT> kraw[NB];
+  V4Block<HD> v4[NB];
+  VRowsRaw<HD, KVT> vr[NB][NI];
+  auto load_v = [&](int b, uint32_t tok) {
     if constexpr (kRows) {
 #pragma unroll
       for (int u = 0; u < NI; ++u) {
         const int i = lane + 64 * u;
-        vr[u].load(a, tok, (i >> 1) % 8, (i & 1) + 2 * (i >> 4));
+        vr[b][u].load(a, tok, (i >> 1) % 8, (i & 1) + 2 * (i >> 4));
       }
     } else {
-#pragma unroll
-      for (int c = 0; c < HD / 64; ++c) v4[c].load(a, tok, c, lane);
+      v4[b].load(a, tok, lane);
     }
   };
-  if (nblk > 0) {
-    find_tokens(0);
-    k.load(a, token(0), lane);
-    load_v(token(0));
-  }
+  // the queries first: loads return in order, and a wait for them behind K and V would drain those too
   u32x4 qf[KS];
   {
-    const uint16_t* src = a.q + ((int64_t)(t.b * a.W + rc / a.G) * a.nq + kvh * a.G + rc % a.G) * HD + 8 * g;
+    const uint16_t* src = a.q + ((int64_t)(t.b * a.W + ri) * a.nq + kvh * a.G + rc - ri * a.G) * HD + 8 * g;
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
   }
   Tile<HD> tile;
   tile.clear();
   uint8_t* vlds = lds + wv * DT * kVTile;
+  if (nstep > 0) {  // the loop within: around it, the count of loads in flight would have to hold for no loads too
+    find_tokens(0);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) kraw[b].load(a, token(0, b), lane);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) load_v(b, token(0, b));
+    int i = 0;
 #pragma unroll 1
-  for (int i = 0; i < nblk; ++i) {
-    const int base = p.base(t.v0 + wv + 4 * i);
-    const bool open = block_open(a, p, base, pos_lo, pos_hi);
-    f32x4 st[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+    do {
+      int base[NB];
+      bool open = true;
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) st[u] = mfma16(k.operand(u, s), qf[s], st[u]);
-    const bool more = i + 1 < nblk;
-    if (more && ((i + 1) & 63) == 0) find_tokens(i + 1);
-    if (more) k.load(a, token(i + 1), lane);
-    if (a.softcap > 0.0f) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) st[u][e] = tanhf(st[u][e] * a.scale / a.softcap) * a.softcap;
-    }
-    if (!open) mask_scores(see, st, 0, base, g);
-    tile.soften(st, c2);
-    u32x4 hi, lo;
-    Tile<HD>::terms(st[0], st[1], hi, lo);
-    u32x4 vf[kRows ? 1 : DT];
-    if constexpr (kRows) {
-#pragma unroll
-      for (int u = 0; u < NI; ++u) {
-        const int it = lane + 64 * u;
-        vr[u].store(a, p, base, (it >> 1) % 8, (it & 1) + 2 * (it >> 4), !open, vlds);
+      for (int b = 0; b < NB; ++b) {
+        const int v = t.v0 + NB * (wv + 4 * i) + b;
+        base[b] = v < t.v1 ? p.base(v) : 0x40000000;  // past the split: no query sees it
+        open &= block_open(a, p, base[b], pos_lo, pos_hi);
       }
-      asm volatile("" ::: "memory");  // a wave's LDS accesses run in order; keep the compiler's order too
-    } else {
+      f32x4 st[2 * NB];
 #pragma unroll
-      for (int c = 0; c < HD / 64; ++c) {
-        if (!open) v4[c].drop_dead(a, p, base, lane);
-        u32x4 x[4];
-        v4[c].operands(x);
+      for (int x = 0; x < 2 * NB; ++x) st[x] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int d = 0; d < 4; ++d) vf[kRows ? 0 : 4 * c + d] = x[d];
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int x = 0; x < 2 * NB; ++x) st[x] = mfma16(kraw[x / 2].operand(x % 2, s), qf[s], st[x]);
+      // the next step's blocks (this one's again at the end: a load that may not happen would have to be
+      // waited for as if it did not)
+      const int nx = min(i + 1, nstep - 1);
+      if (nx > i && (nx & 63) == 0) find_tokens(nx);
+      uint32_t tok_nx[NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        tok_nx[b] = token(nx, b);
+        kraw[b].load(a, tok_nx[b], lane);
       }
-    }
-    if (more) load_v(token(i + 1));
-    auto operand = [&](int d) {
-      if constexpr (kRows) return v_operand(vlds, d, lane);
-      else return vf[kRows ? 0 : d];
-    };
-    bool guarded = false;
-    if (!open) {
-      bool bad = false;
+      if (a.softcap > 0.0f) {
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const u32x4 x = operand(d);
-        bad |= nonfinite2(x[0]) || nonfinite2(x[1]) || nonfinite2(x[2]) || nonfinite2(x[3]);
+        for (int x = 0; x < 2 * NB; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) st[x][e] = tanhf(st[x][e] * a.scale / a.softcap) * a.softcap;
       }
-      guarded = __any(bad);
-    }
+      if (!open) {
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      u32x4 x = operand(d);
-      if (guarded) x = finite_only(x);
-      tile.o[d] = mfma16(x, lo, mfma16(x, hi, tile.o[d]));
-    }
-    if (guarded) {
-      tile.add_nonfinite(see, base, lane, hi, lo, [&](int d, int k, int gg, int rr) -> uint32_t {
-        const int e = (k / 16) * 4 + k % 4, at = 4 * gg + rr + 16 * ((k % 16) / 4);  // the lane that holds it
+        for (int b = 0; b < NB; ++b) mask_scores(see, st, 2 * b, base[b], g);
+      }
+      tile.soften(st, c2);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        u32x4 hi, lo;
+        Tile<HD>::terms(st[2 * b], st[2 * b + 1], hi, lo);
         if constexpr (kRows) {
-          return *reinterpret_cast<const uint16_t*>(vlds + d * kVTile + (at >> 4) * kVGroup + (at & 15) * 16 + 2 * e);
+#pragma unroll
+          for (int u = 0; u < NI; ++u) {
+            const int it = lane + 64 * u;
+            vr[b][u].pin();
+            vr[b][u].store(a, p, base[b], (it >> 1) % 8, (it & 1) + 2 * (it >> 4), !open, vlds);
+          }
+          asm volatile("" ::: "memory");  // a wave's LDS accesses run in order; keep the compiler's order too
         } else {
-          const u32x4& x = vf[kRows ? 0 : d];
-          const uint32_t w = __shfl(e < 4 ? (e < 2 ? x[0] : x[1]) : (e < 6 ? x[2] : x[3]), at, 64);
-          return e & 1 ? w >> 16 : w & 0xffffu;
+          v4[b].pin();
+          if (!open) v4[b].drop_dead(a, p, base[b], lane);
         }
-      });
-    }
-    if constexpr (kRows) asm volatile("" ::: "memory");
+        static_for<DT / 4>([&](auto q) {
+          constexpr int Q = decltype(q)::value, D = 4 * Q;
+          u32x4 y[4];
+          if constexpr (kRows) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d) y[d] = v_operand(vlds, D + d, lane);
+          } else {
+            v4[b].operands(Q, y);
+          }
+          if (!open && any_nonfinite(y)) {
+            tile.template add_nonfinite<D>(see, base[b], lane, hi, lo, [&](int d, int k, int gg, int rr) -> uint32_t {
+              const int e = (k / 16) * 4 + k % 4, at = 4 * gg + rr + 16 * ((k % 16) / 4);  // the lane that holds it
+              if constexpr (kRows) {
+                return *reinterpret_cast<const uint16_t*>(vlds + (D + d) * kVTile + (at >> 4) * kVGroup + (at & 15) * 16 + 2 * e);
+              } else {
+                const u32x4& z = y[d];
+                const uint32_t w = __shfl(e < 4 ? (e < 2 ? z[0] : z[1]) : (e < 6 ? z[2] : z[3]), at, 64);
+                return e & 1 ? w >> 16 : w & 0xffffu;
+              }
+            });
+#pragma unroll
+            for (int d = 0; d < 4; ++d) y[d] = finite_only(y[d]);
+          }
+          tile.template add4<D>(y, hi, lo);
+        });
+        if constexpr (kRows) asm volatile("" ::: "memory");
+        load_v(b, tok_nx[b]);
+      }
+    } while (++i < nstep);
   }
   float l = tile.l;
   l += __shfl_xor(l, 16, 64);
@@ -564,16 +693,27 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const int w4 = wv & 3;
   const bool do_k = NW == 4 || wv < 4, do_v = NW == 4 || wv >= 4;
-  const int kvh = blockIdx.x % a.nkv, group = a.groups - 1 - (int)blockIdx.y;  // the groups with the most keys first
-  const SplitTask t = split_task(a, blockIdx.x / a.nkv, group);
+  const int slot = a.by_nkv.quot(blockIdx.x), kvh = blockIdx.x - slot * a.nkv;
+  const int group = a.groups - 1 - (int)blockIdx.y;  // the groups with the most keys first
+  const SplitTask t = split_task(a, slot, group);
   if (t.live == 0) return;
   const KeyPlan& p = t.p;
   const int r0 = group * a.grows + wv * TPW * 16;
   const bool wave_live = r0 < a.R;
-  const int pos_lo = p.off + min(r0, a.R - 1) / a.G, pos_hi = p.off + (min(r0 + TPW * 16, a.R) - 1) / a.G;
+  const int pos_lo = p.off + a.by_G.quot(min(r0, a.R - 1)), pos_hi = p.off + a.by_G.quot(min(r0 + TPW * 16, a.R) - 1);
   const float c2 = (a.softcap > 0.0f ? 1.0f : a.scale) * kLog2e;
   const int nch = t.v1 > t.v0 ? (t.v1 - t.v0 + NB - 1) / NB : 0;
 
+  u32x4 qf[TPW][KS];
+  Sight see[TPW];
+#pragma unroll
+  for (int u = 0; u < TPW; ++u) {
+    const int rc = min(r0 + 16 * u + n, a.R - 1), ri = a.by_G.quot(rc);
+    see[u] = sight(a, p, p.off + ri);
+    const uint16_t* src = a.q + ((int64_t)(t.b * a.W + ri) * a.nq + kvh * a.G + rc - ri * a.G) * HD + 8 * g;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[u][s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
+  }
   // this thread's pieces of a chunk: K units of (block, tile[, half]) and V units of (block, chunk) for 4-bit
   // codes; 4 K tiles of 16 x 32 and 4 keys x 8 dims of V for rows
   constexpr int kUnits = 4;
@@ -586,8 +726,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
     for (int u = 0; u < NB; ++u) {
       const int base = p.base(min(t.v0 + c * NB + u, t.v1 - 1));
-      const int pg = a.block_table[(int64_t)t.b * a.max_pages + base / a.page];
-      tok_next[u] = ((uint32_t)pg * a.nkv + kvh) * a.page + base % a.page;
+      const int lp = a.by_page.quot(base), pg = a.block_table[(int64_t)t.b * a.max_pages + lp];
+      tok_next[u] = ((uint32_t)pg * a.nkv + kvh) * a.page + (base - lp * a.page);
     }
   };
   // U4 K unit w4: tile w4 (head_dim 128: of 64 keys), or tile w4 / 2, half w4 % 2 (256); V unit: chunk w4 % (HD / 64) of block w4 / (HD / 64)
@@ -653,16 +793,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     }
   };
 
-  u32x4 qf[TPW][KS];
-  Sight see[TPW];
-#pragma unroll
-  for (int u = 0; u < TPW; ++u) {
-    const int rc = min(r0 + 16 * u + n, a.R - 1);
-    see[u] = sight(a, p, p.off + rc / a.G);
-    const uint16_t* src = a.q + ((int64_t)(t.b * a.W + rc / a.G) * a.nq + kvh * a.G + rc % a.G) * HD + 8 * g;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) qf[u][s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
-  }
   Tile<HD> tile[TPW];
 #pragma unroll
   for (int u = 0; u < TPW; ++u) tile[u].clear();
@@ -711,33 +841,24 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
     for (int x = 0; x < NB; ++x) {
       const uint8_t* vb8 = &vbuf[buf][x * DT * kVTile];
-      bool guarded = false;
-      if (!open) {
-        bool bad = false;
+      static_for<DT / 4>([&](auto q) {
+        constexpr int D = 4 * decltype(q)::value;
+        u32x4 w[4];
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const u32x4 w = v_operand(vb8, d, lane);
-          bad |= nonfinite2(w[0]) || nonfinite2(w[1]) || nonfinite2(w[2]) || nonfinite2(w[3]);
+        for (int d = 0; d < 4; ++d) w[d] = v_operand(vb8, D + d, lane);
+        if (!open && any_nonfinite(w)) {
+#pragma unroll
+          for (int u = 0; u < TPW; ++u)
+            tile[u].template add_nonfinite<D>(see[u], base[x], lane, hi[u][x], lo[u][x], [&](int d, int k, int gg, int rr) -> uint32_t {
+              return *reinterpret_cast<const uint16_t*>(vb8 + (D + d) * kVTile + ((k % 16) / 4) * kVGroup + (4 * gg + rr) * 16 +
+                                                        2 * ((k / 16) * 4 + k % 4));
+            });
+#pragma unroll
+          for (int d = 0; d < 4; ++d) w[d] = finite_only(w[d]);
         }
-        guarded = __any(bad);
-      }
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        u32x4 w = v_operand(vb8, d, lane);
-        if (guarded) w = finite_only(w);
-#pragma unroll
-        for (int u = 0; u < TPW; ++u) tile[u].o[d] = mfma16(w, hi[u][x], tile[u].o[d]);
-#pragma unroll
-        for (int u = 0; u < TPW; ++u) tile[u].o[d] = mfma16(w, lo[u][x], tile[u].o[d]);
-      }
-      if (guarded) {
-#pragma unroll
-        for (int u = 0; u < TPW; ++u)
-          tile[u].add_nonfinite(see[u], base[x], lane, hi[u][x], lo[u][x], [&](int d, int k, int gg, int rr) -> uint32_t {
-            return *reinterpret_cast<const uint16_t*>(vb8 + d * kVTile + ((k % 16) / 4) * kVGroup + (4 * gg + rr) * 16 +
-                                                      2 * ((k / 16) * 4 + k % 4));
-          });
-      }
+        for (int u = 0; u < TPW; ++u) tile[u].template add4<D>(w, hi[u][x], lo[u][x]);
+      });
     }
   };
 
@@ -748,18 +869,19 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     stage(0, 0);
     if (nch > 1) issue();
     if (nch > 2) find(2);
-  }
-  __syncthreads();
-#pragma unroll 1
-  for (int c = 0; c < nch; ++c) {
-    compute(c & 1, c);
-    if (c + 1 < nch) {
-      // the other buffer was last read for chunk c - 1, before the last barrier
-      stage((c + 1) & 1, c + 1);
-      if (c + 2 < nch) issue();
-      if (c + 3 < nch) find(c + 3);
-    }
     __syncthreads();
+    int c = 0;
+#pragma unroll 1
+    do {
+      compute(c & 1, c);
+      if (c + 1 < nch) {
+        // the other buffer was last read for chunk c - 1, before the last barrier
+        stage((c + 1) & 1, c + 1);
+        if (c + 2 < nch) issue();
+        if (c + 3 < nch) find(c + 3);
+      }
+      __syncthreads();
+    } while (++c < nch);
   }
 #pragma unroll
   for (int u = 0; u < TPW; ++u) {
@@ -793,7 +915,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(SinkArgs a) {
   constexpr int C = HD / 4, S = 256 / C, U = 4;
   __shared__ f32x4 acc_s[S][C];
   __shared__ float2 ml_s[S];
-  const int r = blockIdx.x % a.R, bk = blockIdx.x / a.R, kvh = bk % a.nkv, b = bk / a.nkv;
+  const int r = blockIdx.x, b = a.by_nkv.quot(blockIdx.y), kvh = blockIdx.y - b * a.nkv;
   const int ch = threadIdx.x % C, sl = threadIdx.x / C;
   int first, live;
   if (a.balanced) {
@@ -803,8 +925,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(SinkArgs a) {
     live = max(1, (key_plan(a, a.seq_lens[b], 0, a.W - 1).T + bps - 1) / bps);
   } else {
     const int group = r / a.grows;
-    const int T = key_plan(a, a.seq_lens[b], group * a.grows / a.G, (min(a.R, (group + 1) * a.grows) - 1) / a.G).T;
-    const int bps = max(kMinSplitBlocks, round4((T + a.nsplit - 1) / a.nsplit));
+    const int T = key_plan(a, a.seq_lens[b], a.by_G.quot(group * a.grows), a.by_G.quot(min(a.R, (group + 1) * a.grows) - 1)).T;
+    const int bps = even_blocks(a, T);
     first = b * a.nsplit;
     live = max(1, (T + bps - 1) / bps);
   }
@@ -864,7 +986,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(SinkArgs a) {
 struct SinkPlan {
   bool tile;       // one tile of rows per workgroup, or blocks of rows
   int waves, tpw;  // block kernel
-  int groups, grows, nsplit, balanced, slots;
+  int groups, grows, nsplit, balanced, slots, unit;
 };
 static SinkPlan sink_plan(int B, int W, int nq, int nkv, int hd, int causal, int window, int sinks, int max_ctx) {
   SinkPlan s = {};
@@ -877,14 +999,16 @@ static SinkPlan sink_plan(int B, int W, int nq, int nkv, int hd, int causal, int
   }
   s.grows = s.tile ? 16 : s.waves * s.tpw * 16;
   s.groups = (int)ceil_div(R, s.grows);
+  s.unit = s.tile ? 4 * (hd == 128 ? kTileBlocks<128> : kTileBlocks<256>) : 4;  // a step of each wave; two chunks of 64 keys
   // blocks of 32 keys a pass may look at (the sliding window's rows, and its sinks)
   int64_t span = max_ctx;
   if (causal && window > 0) span = std::min<int64_t>(span, (int64_t)window + W + sinks + 96);
-  const int64_t most = std::max<int64_t>(1, ceil_div(ceil_div(span, 32) + 1, kMinSplitBlocks));
-  const int64_t tasks = (int64_t)B * nkv * s.groups, want = 512;
+  const int64_t most = std::max<int64_t>(1, ceil_div(ceil_div(span, 32) + 1, s.unit));
+  // workgroups that run at once: two per CU, one of the tile kernel at head_dim 256 (its registers)
+  const int64_t tasks = (int64_t)B * nkv * s.groups, want = s.tile && hd == 256 ? 256 : 512;
   s.nsplit = (int)std::min<int64_t>(most, std::max<int64_t>(1, want / tasks));
   s.balanced = s.groups == 1 && B <= kBalancedRows && B > 1 && s.nsplit > 1;
-  s.slots = s.balanced ? B * s.nsplit + B : B * s.nsplit;
+  s.slots = B * s.nsplit;
   return s;
 }
 static size_t sink_part_o_bytes(const SinkPlan& s, int64_t R, int nkv, int hd) {
@@ -905,7 +1029,7 @@ static void launch_sinks(const SinkArgs& a, const SinkPlan& s, hipStream_t st) {
     hipLaunchKernelGGL((attention_block_kernel<HD, KVT, 4, 1>), grid, dim3(256), 0, st, a);
   }
   if (s.nsplit > 1)
-    hipLaunchKernelGGL((attention_join_kernel<HD>), dim3((unsigned)((int64_t)a.B * a.nkv * a.R)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attention_join_kernel<HD>), dim3((unsigned)a.R, (unsigned)(a.B * a.nkv)), dim3(256), 0, st, a);
 }
 
 }  // namespace dsk
@@ -942,7 +1066,7 @@ extern "C" int dsk_attention_sinks(const uint16_t* q, int B, int W, int nq, int 
   DSK_REQUIRE(!out_packed || (B * W <= 64 && (nq * hd) % 64 == 0), "%s: packed output needs B*W <= 64", who);
   const int64_t R = (int64_t)W * (nq / nkv);
   const SinkPlan s = sink_plan(B, W, nq, nkv, hd, causal, window, sinks, max_ctx);
-  DSK_REQUIRE(R <= 0x7fffffff && s.groups <= 65535 && (int64_t)s.slots * nkv <= 0x7fffffff && (int64_t)B * nkv * R <= 0x7fffffff,
+  DSK_REQUIRE(R <= 0x7fffffff && s.groups <= 65535 && (int64_t)s.slots * nkv <= 0x7fffffff && (int64_t)B * nkv <= 65535,
               "%s: %lld query rows per kv head", who, (long long)R);
   const size_t need = sink_ws(s, R, nkv, hd);
   if (need && (!workspace || ws_bytes < need)) {
@@ -952,8 +1076,9 @@ extern "C" int dsk_attention_sinks(const uint16_t* q, int B, int W, int nq, int 
   DSK_REQUIRE(((uintptr_t)workspace & 15) == 0 || need == 0, "%s: workspace must be 16-byte aligned", who);
   SinkArgs a = {q, B, W, nq, nkv, nq / nkv, (int)R, scale, softcap, causal ? 1 : 0, window, sinks, seq_lens, block_table,
                 max_pages, page, k_pool, v_pool, k_sb, v_sb, out, out_packed ? 1 : 0, s.groups, s.grows, s.slots, s.nsplit,
-                s.balanced, reinterpret_cast<float*>(workspace),
-                reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + sink_part_o_bytes(s, R, nkv, hd))};
+                s.balanced, s.unit, reinterpret_cast<float*>(workspace),
+                reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + sink_part_o_bytes(s, R, nkv, hd)),
+                FastDiv(page), FastDiv(nq / nkv), FastDiv(nkv), FastDiv(s.nsplit)};
 #define DSK_SINKS(HDV)                                                                                \
   if (kv_dtype == DSK_KV_BF16) launch_sinks<HDV, DSK_KV_BF16>(a, s, as_stream(stream));               \
   else if (kv_dtype == DSK_KV_U8) launch_sinks<HDV, DSK_KV_U8>(a, s, as_stream(stream));              \

@@ -37,7 +37,9 @@ struct Kv4Scale {
   float s24, s20, b;
 };
 __device__ __forceinline__ Kv4Scale kv4_scale(uint32_t w) {
-  return Kv4Scale{bits_f32((w << 16) + (24u << 23)), bits_f32((w << 16) + (20u << 23)), bits_f32(w & 0xffff0000u)};
+  uint32_t s24;  // one instruction, which the compiler splits into two to share the shift
+  asm("v_lshl_add_u32 %0, %1, 16, %2" : "=v"(s24) : "v"(w), "s"(24u << 23));
+  return Kv4Scale{bits_f32(s24), bits_f32(s24 - (4u << 23)), bits_f32(w & 0xffff0000u)};
 }
 
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));

@@ -144,15 +144,21 @@ def call(name: str, *args) -> None:
 
 
 def stream_ptr():
-    """The current torch (HIP) stream as a raw hipStream_t."""
+    """The current torch (HIP) stream as a raw hipStream_t (without building a torch.cuda.Stream: 0.3 us
+    against 3)."""
     import torch
 
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def ptr(t) -> C.c_void_p:
     """Device pointer of a torch tensor (None -> NULL)."""
     return C.c_void_p(0 if t is None else t.data_ptr())
+
+
+def addr(t):
+    """ptr as the plain integer (or None) that ctypes converts by itself: half the time per argument."""
+    return None if t is None else t.data_ptr()
 
 
 def exported_symbols() -> list[str]:

@@ -8,6 +8,7 @@ tensors must live on a HIP device.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import math
 from dataclasses import dataclass
@@ -16,7 +17,7 @@ import torch
 
 from . import _hip
 from ._hip import (DSK_BF16, DSK_EPI_GEGLU, DSK_EPI_PARTIAL, DSK_EPI_RESIDUAL, DSK_EPI_STORE, DSK_EPI_SWIGLU, DSK_F32,
-                   DSK_KV_BF16, DSK_KV_U4, DSK_KV_U8, call, ptr, stream_ptr)
+                   DSK_KV_BF16, DSK_KV_U4, DSK_KV_U8, addr, call, ptr, stream_ptr)
 
 __all__ = [
     "W8Weight", "W8Table", "Workspace", "Packed", "act_pack", "pack", "pack_rn", "w8_gemm", "w8_residual", "w8_embed",
@@ -513,9 +514,14 @@ def kv_read(first, n, nkv, hd, block_table, page, kv_dtype, k_pool, v_pool, k_sb
     if n == 0:
         return tuple(outs)
     _on_device(k_pool)
-    call("dsk_kv_read", ptr(first), int(offset), B, int(n), nkv, hd, ptr(block_table), block_table.shape[1], page,
-         kv_dtype, ptr(k_pool), ptr(v_pool), ptr(k_sb), ptr(v_sb), ptr(outs[0]), ptr(outs[1]), stream_ptr())
+    call("dsk_kv_read", addr(first), offset, B, n, nkv, hd, addr(block_table), block_table.shape[1], page, kv_dtype,
+         addr(k_pool), addr(v_pool), addr(k_sb), addr(v_sb), addr(outs[0]), addr(outs[1]), stream_ptr())
     return tuple(outs)
+
+
+@functools.lru_cache(maxsize=4096)
+def _sinks_ws_bytes(*args) -> int:
+    return _hip.lib.dsk_attention_sinks_ws_bytes(*args)
 
 
 def attention(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table, page, kv_dtype, k_pool,
@@ -534,14 +540,13 @@ def attention(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table, page,
         if odata.dtype != torch.bfloat16 or not odata.is_contiguous() or (
                 not isinstance(out, Packed) and odata.numel() != B * W * nq * hd):
             raise ValueError(f"attention: out must be contiguous bf16 [{B * W}, {nq * hd}]")
-        need = _hip.lib.dsk_attention_sinks_ws_bytes(B, W, nq, nkv, hd, int(bool(causal)), int(window), int(sinks),
-                                                     int(max_ctx))
+        args = (B, W, nq, nkv, hd, int(bool(causal)), int(window), int(sinks), int(max_ctx))
+        need = _sinks_ws_bytes(*args)
         # per call: passes on two streams, or of two captured graphs, may overlap
         buf = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        call("dsk_attention_sinks", ptr(q), B, W, nq, nkv, hd, float(scale), int(bool(causal)), int(window),
-             int(sinks), float(softcap), ptr(seq_lens), int(max_ctx), ptr(block_table), block_table.shape[1], page,
-             kv_dtype, ptr(k_pool), ptr(v_pool), ptr(k_sb), ptr(v_sb), ptr(odata), int(isinstance(out, Packed)),
-             ptr(buf), need, stream_ptr())
+        call("dsk_attention_sinks", addr(q), *args[:5], scale, *args[5:8], softcap, addr(seq_lens), args[8],
+             addr(block_table), block_table.shape[1], page, kv_dtype, addr(k_pool), addr(v_pool), addr(k_sb),
+             addr(v_sb), addr(odata), int(isinstance(out, Packed)), addr(buf), need, stream_ptr())
         return out
     ws = Workspace.get(q.device)
     need = _hip.lib.dsk_attn_ws_bytes(B, W, nq, hd, max_ctx)
