@@ -29,6 +29,8 @@ struct FastDiv {
   __device__ __forceinline__ int quot(int x) const { return (int)((__umulhi((uint32_t)x, m) + (uint32_t)x) >> s); }
 };
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 struct SinkArgs {
   const uint16_t* q;  // [B*W][nq*HD]
   int B, W, nq, nkv, G, R;  // R = W * G query rows per (row b, kv head)
@@ -45,13 +47,13 @@ struct SinkArgs {
   int grows;     // rows per group
   int slots;     // splits on the grid per kv head: placed by the rows' lengths (balanced), or nsplit for each row
   int nsplit, balanced;
-  int unit;        // splits are multiples of this many 32-key blocks (a power of two)
   float* part_o;   // [slot][kv head][R][HD] unnormalised outputs
   float* part_ml;  // [slot][kv head][R][2] running maximum (of scores times c2) and sum
   FastDiv by_page, by_G, by_nkv, by_nsplit;
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kSplitUnit = 4;       // splits are multiples of this many 32-key blocks: one per wave, or two chunks of 64
 constexpr float kMaxSlack = 8.0f;   // how far (log2) a score may pass the running maximum
 constexpr int kBalancedRows = 64;   // rows whose lengths a workgroup reads to place its split
 
@@ -82,24 +84,26 @@ struct SplitTask {
   int b, slot, v0, v1, live;
   KeyPlan p;
 };
-__device__ __forceinline__ int balanced_blocks(const SinkArgs& a) {
+// The rows' lengths, one per lane (one load for all: read one after the other they cost a round trip each).
+__device__ __forceinline__ int row_lengths(const SinkArgs& a) { return a.seq_lens[min((int)(threadIdx.x & 63), a.B - 1)]; }
+__device__ __forceinline__ int balanced_blocks(const SinkArgs& a, int lens) {
   int total = 0;
-  for (int b = 0; b < a.B; ++b) total += key_plan(a, a.seq_lens[b], 0, a.W - 1).T;
+  for (int b = 0; b < a.B; ++b) total += key_plan(a, __builtin_amdgcn_readlane(lens, b), 0, a.W - 1).T;
   // sum of ceil(T / bps) <= (slots - B) + B
-  return max(a.unit, ((total + a.slots - a.B - 1) / (a.slots - a.B) + a.unit - 1) & -a.unit);
+  return max(kSplitUnit, ((total + a.slots - a.B - 1) / (a.slots - a.B) + kSplitUnit - 1) & -kSplitUnit);
 }
 __device__ __forceinline__ int even_blocks(const SinkArgs& a, int T) {
-  return max(a.unit, (a.by_nsplit.quot(T + a.nsplit - 1) + a.unit - 1) & -a.unit);
+  return max(kSplitUnit, (a.by_nsplit.quot(T + a.nsplit - 1) + kSplitUnit - 1) & -kSplitUnit);
 }
 __device__ __forceinline__ SplitTask split_task(const SinkArgs& a, int slot, int group) {
   SplitTask t;
   t.slot = slot;
   t.live = 0;
   if (a.balanced) {
-    const int bps = balanced_blocks(a);
+    const int lens = row_lengths(a), bps = balanced_blocks(a, lens);
     int first = 0;
     for (int b = 0; b < a.B; ++b) {
-      const KeyPlan p = key_plan(a, a.seq_lens[b], 0, a.W - 1);
+      const KeyPlan p = key_plan(a, __builtin_amdgcn_readlane(lens, b), 0, a.W - 1);
       const int live = max(1, (p.T + bps - 1) / bps);
       if (slot < first + live) {
         t.b = b;
@@ -279,16 +283,16 @@ __device__ __forceinline__ void mask_scores(const Sight& see, f32x4 (&st)[NKT], 
   }
 }
 
-// the words of bf16(s c + b) of 8 consecutive dims of an 8-bit row
-__device__ __forceinline__ u32x4 kv8_row8(uint2 r, uint32_t z) {
-  const float s = bits_f32(z << 16), b = bits_f32(z & 0xffff0000u);
-  u32x4 w;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t two = (e < 2 ? r.x : r.y) >> (16 * (e & 1));
-    w[e] = pack_bf16x2(fmaf(s, (float)(two & 255), b), fmaf(s, (float)((two >> 8) & 255), b));
-  }
-  return w;
+// 4 codes of an 8-bit row -> two words of bf16(s c + b), c as a float16 denormal (kv4.h): 4.1 ns of a SIMD per
+// code at two waves where v_cvt_f32_ubyte and an fma take 5.4
+__device__ __forceinline__ u32x2 kv8_row4(uint32_t w, float s24, float b) {
+  const uint32_t x = w & 0x00ff00ffu, y = (w >> 8) & 0x00ff00ffu;
+  return u32x2{pack_bf16x2(kv4_lo(x, s24, b), kv4_lo(y, s24, b)), pack_bf16x2(kv4_hi(x, s24, b), kv4_hi(y, s24, b))};
+}
+__device__ __forceinline__ u32x4 kv8_row8(uint32_t w0, uint32_t w1, uint32_t z) {
+  const Kv4Scale k = kv4_scale(z);
+  const u32x2 a = kv8_row4(w0, k.s24, k.b), b = kv8_row4(w1, k.s24, k.b);
+  return u32x4{a[0], a[1], b[0], b[1]};
 }
 
 // ----------------------------------------------------------------------------- K and V of a block
@@ -296,13 +300,11 @@ __device__ __forceinline__ u32x4 kv8_row8(uint2 r, uint32_t z) {
 // meanwhile), and the operands they become.
 // Every member is one load: parts of a wider load held in separate variables would be copied (and so
 // waited for) where the loop comes round.
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 // K: u32x4 per 16-key tile and 32-dim step (A operand of the score product).
 template <int HD, int KVT>
 struct KRaw {
   static constexpr bool kBytes = KVT == DSK_KV_U8;
-  u32x4 q[2][KVT == DSK_KV_BF16 ? HD / 32 : (kBytes ? 1 : HD / 128)];
-  u32x2 h[2][kBytes ? HD / 32 : 1];  // 8-bit: 8 dims of each step
+  u32x4 q[2][KVT == DSK_KV_BF16 ? HD / 32 : (kBytes ? HD / 64 : HD / 128)];
   u32x2 sb[2][KVT == DSK_KV_BF16 ? 1 : HD / 128];
   // tok: pool token of the block's first key
   __device__ __forceinline__ void load(const SinkArgs& a, uint32_t tok, int lane) {
@@ -315,9 +317,9 @@ struct KRaw {
 #pragma unroll
         for (int s = 0; s < HD / 32; ++s) q[t][s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
       } else if constexpr (kBytes) {
-        const uint8_t* src = reinterpret_cast<const uint8_t*>(a.k_pool) + row * HD + 8 * g;
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(a.k_pool) + row * HD + 16 * g;
 #pragma unroll
-        for (int s = 0; s < HD / 32; ++s) h[t][s] = *reinterpret_cast<const u32x2*>(src + 32 * s);
+        for (int s = 0; s < HD / 64; ++s) q[t][s] = *reinterpret_cast<const u32x4*>(src + 64 * s);
       } else {
         const uint8_t* src = reinterpret_cast<const uint8_t*>(a.k_pool) + row * (HD / 2) + 16 * g;
 #pragma unroll
@@ -329,9 +331,12 @@ struct KRaw {
       }
     }
   }
+  // first of the 8 dims that step s takes from lane group g (the queries come in the same order): an 8-bit
+  // row's lane holds 16 consecutive dims for two steps
+  static __device__ __forceinline__ int dim(int s, int g) { return kBytes ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g; }
   __device__ __forceinline__ u32x4 operand(int t, int s) const {
     if constexpr (KVT == DSK_KV_BF16) return q[t][s];
-    else if constexpr (kBytes) return kv8_row8(uint2{h[t][s][0], h[t][s][1]}, sb[t][s / 4][(s / 2) & 1]);
+    else if constexpr (kBytes) return kv8_row8(q[t][s / 2][2 * (s & 1)], q[t][s / 2][2 * (s & 1) + 1], sb[t][s / 4][(s / 2) & 1]);
     else return kv4_row8(q[t][s / 4][s % 4], kv4_scale(sb[t][s / 4][(s / 2) & 1]));
   }
 };
@@ -422,53 +427,61 @@ struct V4Block {
   }
 };
 
-// row-major V (bf16, 8-bit): 4 keys x 8 dims, transposed on their way into the operand order in LDS
-template <int HD, int KVT>
+// row-major V (bf16, 8-bit): 4 keys x C dims (8, or 16 of 8 bits), transposed on their way into the operand
+// order in LDS
+template <int HD, int KVT, int C = 8>
 struct VRowsRaw {
   static constexpr bool kBytes = KVT == DSK_KV_U8;
-  u32x4 q[kBytes ? 1 : 4];
-  u32x2 h[kBytes ? 4 : 1];
+  static_assert(C == 8 || (kBytes && C == 16), "one 8- or 16-byte load per key");
+  u32x4 q[C == 16 || !kBytes ? 4 : 1];
+  u32x2 h[kBytes && C == 8 ? 4 : 1];
   uint32_t sb[4];
-  // quad: keys 4 quad .. + 3 of the block, ch: dims 8 ch .. + 7
+  // quad: keys 4 quad .. + 3 of the block, ch: dims C ch .. + C - 1
   __device__ __forceinline__ void load(const SinkArgs& a, uint32_t tok, int quad, int ch) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int64_t row = (int64_t)tok + 4 * quad + r;
-      if constexpr (KVT == DSK_KV_BF16) {
+      if constexpr (!kBytes) {
         q[r] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(a.v_pool) + row * HD + 8 * ch);
       } else {
-        h[r] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint8_t*>(a.v_pool) + row * HD + 8 * ch);
-        sb[r] = a.v_sb[row * (HD / 64) + ch / 8];
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(a.v_pool) + row * HD + C * ch;
+        if constexpr (C == 16) q[r] = *reinterpret_cast<const u32x4*>(src);
+        else h[r] = *reinterpret_cast<const u32x2*>(src);
+        sb[r] = a.v_sb[row * (HD / 64) + ch / (64 / C)];
       }
     }
   }
   // not used before this point: the scheduler would otherwise turn V into operands (and wait for it) while
   // the scores are still on their way
   __device__ __forceinline__ void pin() {
-    if constexpr (kBytes) {
-      asm volatile("" : "+v"(h[0]), "+v"(h[1]), "+v"(h[2]), "+v"(h[3]));
-      asm volatile("" : "+v"(sb[0]), "+v"(sb[1]), "+v"(sb[2]), "+v"(sb[3]));
-    } else {
-      asm volatile("" : "+v"(q[0]), "+v"(q[1]), "+v"(q[2]), "+v"(q[3]));
-    }
+    if constexpr (C == 16 || !kBytes) asm volatile("" : "+v"(q[0]), "+v"(q[1]), "+v"(q[2]), "+v"(q[3]));
+    else asm volatile("" : "+v"(h[0]), "+v"(h[1]), "+v"(h[2]), "+v"(h[3]));
+    if constexpr (kBytes) asm volatile("" : "+v"(sb[0]), "+v"(sb[1]), "+v"(sb[2]), "+v"(sb[3]));
   }
   // base: the block's first key; dst: the block's operands in LDS
   __device__ __forceinline__ void store(const SinkArgs& a, const KeyPlan& p, int base, int quad, int ch, bool check,
                                         uint8_t* dst) const {
-    u32x4 w[4];
+    uint32_t keep[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if constexpr (kBytes) w[r] = kv8_row8(uint2{h[r][0], h[r][1]}, sb[r]);
-      else w[r] = q[r];
-      const uint32_t keep = check && key_dead(a, p, base + 4 * quad + r) ? 0u : ~0u;
-      w[r] &= u32x4{keep, keep, keep, keep};
-    }
-    uint8_t* o = dst + (ch / 2) * kVTile + (quad % 4) * kVGroup + (ch % 2) * 128 + (quad / 4) * 8;
+    for (int r = 0; r < 4; ++r) keep[r] = check && key_dead(a, p, base + 4 * quad + r) ? 0u : ~0u;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-      *reinterpret_cast<uint2*>(o + 16 * e) = uint2{__builtin_amdgcn_perm(w[1][e / 2], w[0][e / 2], sel),
-                                                    __builtin_amdgcn_perm(w[3][e / 2], w[2][e / 2], sel)};
+    for (int half = 0; half < C / 8; ++half) {
+      const int ch8 = C / 8 * ch + half;
+      u32x4 w[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (!kBytes) w[r] = q[r];
+        else if constexpr (C == 16) w[r] = kv8_row8(q[r][2 * half], q[r][2 * half + 1], sb[r]);
+        else w[r] = kv8_row8(h[r][0], h[r][1], sb[r]);
+        w[r] &= u32x4{keep[r], keep[r], keep[r], keep[r]};
+      }
+      uint8_t* o = dst + (ch8 / 2) * kVTile + (quad % 4) * kVGroup + (ch8 % 2) * 128 + (quad / 4) * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+        *reinterpret_cast<uint2*>(o + 16 * e) = uint2{__builtin_amdgcn_perm(w[1][e / 2], w[0][e / 2], sel),
+                                                      __builtin_amdgcn_perm(w[3][e / 2], w[2][e / 2], sel)};
+      }
     }
   }
 };
@@ -481,18 +494,12 @@ __device__ __forceinline__ u32x4 v_operand(const uint8_t* blk, int d, int lane) 
 // One tile of 16 query rows per workgroup; its split's blocks go round its four waves, each with a running
 // state of its own, merged in LDS at the end. No barrier before that: a wave turns its own loads into its
 // own operands (4-bit V lies in operand order; row-major V is transposed through the wave's LDS).
-// Page ids of 64 steps' blocks are loaded at once, one per lane.
-//
-// Bound by the instructions that turn codes into operands (17 for 8 codes: at 2 waves per SIMD a
-// v_fma_mix_f32 or v_cvt_pk takes 2.1 ns of a SIMD, a v_and or v_fma 1.3), not by memory. A step is NB
-// blocks: with one, the chain from scores to probabilities has too few independent instructions to hide
-// its latencies behind.
-template <int HD> constexpr int kTileBlocks = HD == 128 ? 2 : 1;  // registers
+// Page ids of 64 blocks are loaded at once, one per lane.
 
 template <int HD, int KVT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 2 : 1, 2))) void attention_tile_kernel(SinkArgs a) {
-  constexpr int KS = HD / 32, DT = HD / 16, NI = HD / 128 * 2;  // NI: (quad, chunk) items per lane
-  constexpr int NB = kTileBlocks<HD>;
+  constexpr int KS = HD / 32, DT = HD / 16;
+  constexpr int VC = KVT == DSK_KV_U8 ? 16 : 8, NI = HD / VC / 8;  // V items (4 keys x VC dims) per lane
   constexpr bool kRows = KVT != DSK_KV_U4;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kRows && 4 * DT * kVTile > 4 * DT * 1024 ? 4 * DT * kVTile : 4 * DT * 1024];
   __shared__ float2 wml[4][16];
@@ -507,134 +514,110 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ?
   const float c2 = (a.softcap > 0.0f ? 1.0f : a.scale) * kLog2e;
   const Sight see = sight(a, p, pos);
 
-  // this wave's steps: blocks v0 + NB (wv + 4 i) .. + NB - 1
-  const int left = t.v1 - t.v0 - NB * wv, nstep = left > 0 ? (left + 4 * NB - 1) / (4 * NB) : 0;
-  uint32_t toks[NB];  // lane l: pool tokens of the blocks of step (i & ~63) + l (past the split: its last block)
+  const int nblk = t.v1 > t.v0 + wv ? (t.v1 - t.v0 - wv + 3) / 4 : 0;  // this wave's blocks v0 + wv + 4 i
+  uint32_t toks = 0;  // lane l: pool token of block (i & ~63) + l
   auto find_tokens = [&](int i) {
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int base = p.base(min(t.v0 + NB * (wv + 4 * (i + lane)) + b, t.v1 - 1));
-      const int lp = a.by_page.quot(base), pg = a.block_table[(int64_t)t.b * a.max_pages + lp];
-      toks[b] = ((uint32_t)pg * a.nkv + kvh) * a.page + (base - lp * a.page);
-    }
+    const int base = p.base(min(t.v0 + wv + 4 * (i + lane), t.v1 - 1));
+    const int lp = a.by_page.quot(base), pg = a.block_table[(int64_t)t.b * a.max_pages + lp];
+    toks = ((uint32_t)pg * a.nkv + kvh) * a.page + (base - lp * a.page);
   };
-  auto token = [&](int i, int b) { return (uint32_t)__builtin_amdgcn_readlane(toks[b], i & 63); };
+  auto token = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane(toks, i & 63); };
 
-  KRaw<HD, KVT> kraw[NB];
-  V4Block<HD> v4[NB];
-  VRowsRaw<HD, KVT> vr[NB][NI];
-  auto load_v = [&](int b, uint32_t tok) {
+  KRaw<HD, KVT> kraw;
+  V4Block<HD> v4;
+  VRowsRaw<HD, KVT, VC> vr[NI];
+  auto quad_of = [](int it) { return (it >> 1) % 8; };  // the bank conflicts of the transposing writes are least so
+  auto chunk_of = [](int it) { return (it & 1) + 2 * (it >> 4); };
+  auto load_v = [&](uint32_t tok) {
     if constexpr (kRows) {
 #pragma unroll
       for (int u = 0; u < NI; ++u) {
-        const int i = lane + 64 * u;
-        vr[b][u].load(a, tok, (i >> 1) % 8, (i & 1) + 2 * (i >> 4));
+        vr[u].load(a, tok, quad_of(lane + 64 * u), chunk_of(lane + 64 * u));
       }
     } else {
-      v4[b].load(a, tok, lane);
+      v4.load(a, tok, lane);
     }
   };
   // the queries first: loads return in order, and a wait for them behind K and V would drain those too
   u32x4 qf[KS];
   {
-    const uint16_t* src = a.q + ((int64_t)(t.b * a.W + ri) * a.nq + kvh * a.G + rc - ri * a.G) * HD + 8 * g;
+    const uint16_t* src = a.q + ((int64_t)(t.b * a.W + ri) * a.nq + kvh * a.G + rc - ri * a.G) * HD;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(src + KRaw<HD, KVT>::dim(s, g));
   }
   Tile<HD> tile;
   tile.clear();
   uint8_t* vlds = lds + wv * DT * kVTile;
-  if (nstep > 0) {  // the loop within: around it, the count of loads in flight would have to hold for no loads too
+  if (nblk > 0) {  // the loop within: around it, the count of loads in flight would have to hold for no loads too
     find_tokens(0);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) kraw[b].load(a, token(0, b), lane);
+    kraw.load(a, token(0), lane);
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) load_v(b, token(0, b));
+    load_v(token(0));
     int i = 0;
 #pragma unroll 1
     do {
-      int base[NB];
-      bool open = true;
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int v = t.v0 + NB * (wv + 4 * i) + b;
-        base[b] = v < t.v1 ? p.base(v) : 0x40000000;  // past the split: no query sees it
-        open &= block_open(a, p, base[b], pos_lo, pos_hi);
-      }
-      f32x4 st[2 * NB];
-#pragma unroll
-      for (int x = 0; x < 2 * NB; ++x) st[x] = f32x4{0, 0, 0, 0};
+      const int base = p.base(t.v0 + wv + 4 * i);
+      const bool open = block_open(a, p, base, pos_lo, pos_hi);
+      f32x4 st[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int x = 0; x < 2 * NB; ++x) st[x] = mfma16(kraw[x / 2].operand(x % 2, s), qf[s], st[x]);
-      // the next step's blocks (this one's again at the end: a load that may not happen would have to be
-      // waited for as if it did not)
-      const int nx = min(i + 1, nstep - 1);
+        for (int x = 0; x < 2; ++x) st[x] = mfma16(kraw.operand(x, s), qf[s], st[x]);
+      // the next block (this one again at the end: a load that may not happen would have to be waited for as
+      // if it did not)
+      const int nx = min(i + 1, nblk - 1);
       if (nx > i && (nx & 63) == 0) find_tokens(nx);
-      uint32_t tok_nx[NB];
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        tok_nx[b] = token(nx, b);
-        kraw[b].load(a, tok_nx[b], lane);
-      }
+      const uint32_t tok_nx = token(nx);
+      kraw.load(a, tok_nx, lane);
       if (a.softcap > 0.0f) {
 #pragma unroll
-        for (int x = 0; x < 2 * NB; ++x)
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int e = 0; e < 4; ++e) st[x][e] = tanhf(st[x][e] * a.scale / a.softcap) * a.softcap;
       }
-      if (!open) {
-#pragma unroll
-        for (int b = 0; b < NB; ++b) mask_scores(see, st, 2 * b, base[b], g);
-      }
+      if (!open) mask_scores(see, st, 0, base, g);
       tile.soften(st, c2);
+      u32x4 hi, lo;
+      Tile<HD>::terms(st[0], st[1], hi, lo);
+      if constexpr (kRows) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        u32x4 hi, lo;
-        Tile<HD>::terms(st[2 * b], st[2 * b + 1], hi, lo);
+        for (int u = 0; u < NI; ++u) {
+          vr[u].pin();
+          vr[u].store(a, p, base, quad_of(lane + 64 * u), chunk_of(lane + 64 * u), !open, vlds);
+        }
+        asm volatile("" ::: "memory");  // a wave's LDS accesses run in order; keep the compiler's order too
+      } else {
+        v4.pin();
+        if (!open) v4.drop_dead(a, p, base, lane);
+      }
+      static_for<DT / 4>([&](auto q) {
+        constexpr int Q = decltype(q)::value, D = 4 * Q;
+        u32x4 y[4];
         if constexpr (kRows) {
 #pragma unroll
-          for (int u = 0; u < NI; ++u) {
-            const int it = lane + 64 * u;
-            vr[b][u].pin();
-            vr[b][u].store(a, p, base[b], (it >> 1) % 8, (it & 1) + 2 * (it >> 4), !open, vlds);
-          }
-          asm volatile("" ::: "memory");  // a wave's LDS accesses run in order; keep the compiler's order too
+          for (int d = 0; d < 4; ++d) y[d] = v_operand(vlds, D + d, lane);
         } else {
-          v4[b].pin();
-          if (!open) v4[b].drop_dead(a, p, base[b], lane);
+          v4.operands(Q, y);
         }
-        static_for<DT / 4>([&](auto q) {
-          constexpr int Q = decltype(q)::value, D = 4 * Q;
-          u32x4 y[4];
-          if constexpr (kRows) {
+        if (!open && any_nonfinite(y)) {
+          tile.template add_nonfinite<D>(see, base, lane, hi, lo, [&](int d, int k, int gg, int rr) -> uint32_t {
+            const int e = (k / 16) * 4 + k % 4, at = 4 * gg + rr + 16 * ((k % 16) / 4);  // the lane that holds it
+            if constexpr (kRows) {
+              return *reinterpret_cast<const uint16_t*>(vlds + (D + d) * kVTile + (at >> 4) * kVGroup + (at & 15) * 16 + 2 * e);
+            } else {
+              const u32x4& z = y[d];
+              const uint32_t w = __shfl(e < 4 ? (e < 2 ? z[0] : z[1]) : (e < 6 ? z[2] : z[3]), at, 64);
+              return e & 1 ? w >> 16 : w & 0xffffu;
+            }
+          });
 #pragma unroll
-            for (int d = 0; d < 4; ++d) y[d] = v_operand(vlds, D + d, lane);
-          } else {
-            v4[b].operands(Q, y);
-          }
-          if (!open && any_nonfinite(y)) {
-            tile.template add_nonfinite<D>(see, base[b], lane, hi, lo, [&](int d, int k, int gg, int rr) -> uint32_t {
-              const int e = (k / 16) * 4 + k % 4, at = 4 * gg + rr + 16 * ((k % 16) / 4);  // the lane that holds it
-              if constexpr (kRows) {
-                return *reinterpret_cast<const uint16_t*>(vlds + (D + d) * kVTile + (at >> 4) * kVGroup + (at & 15) * 16 + 2 * e);
-              } else {
-                const u32x4& z = y[d];
-                const uint32_t w = __shfl(e < 4 ? (e < 2 ? z[0] : z[1]) : (e < 6 ? z[2] : z[3]), at, 64);
-                return e & 1 ? w >> 16 : w & 0xffffu;
-              }
-            });
-#pragma unroll
-            for (int d = 0; d < 4; ++d) y[d] = finite_only(y[d]);
-          }
-          tile.template add4<D>(y, hi, lo);
-        });
-        if constexpr (kRows) asm volatile("" ::: "memory");
-        load_v(b, tok_nx[b]);
-      }
-    } while (++i < nstep);
+          for (int d = 0; d < 4; ++d) y[d] = finite_only(y[d]);
+        }
+        tile.template add4<D>(y, hi, lo);
+      });
+      if constexpr (kRows) asm volatile("" ::: "memory");
+      load_v(tok_nx);
+    } while (++i < nblk);
   }
   float l = tile.l;
   l += __shfl_xor(l, 16, 64);
@@ -767,7 +750,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
           u32x4 w = kq[u];
-          if constexpr (KVT == DSK_KV_U8) w = kv8_row8(uint2{kq[u][0], kq[u][1]}, ksb[u]);
+          if constexpr (KVT == DSK_KV_U8) w = kv8_row8(kq[u][0], kq[u][1], ksb[u]);
           *reinterpret_cast<u32x4*>(&kbuf[buf][(w4 * kUnits + u) * 1024 + lane * 16]) = w;
         }
       } else {
@@ -919,10 +902,10 @@ __global__ __launch_bounds__(256) void attention_join_kernel(SinkArgs a) {
   const int ch = threadIdx.x % C, sl = threadIdx.x / C;
   int first, live;
   if (a.balanced) {
-    const int bps = balanced_blocks(a);
+    const int lens = row_lengths(a), bps = balanced_blocks(a, lens);
     first = 0;
-    for (int x = 0; x < b; ++x) first += max(1, (key_plan(a, a.seq_lens[x], 0, a.W - 1).T + bps - 1) / bps);
-    live = max(1, (key_plan(a, a.seq_lens[b], 0, a.W - 1).T + bps - 1) / bps);
+    for (int x = 0; x < b; ++x) first += max(1, (key_plan(a, __builtin_amdgcn_readlane(lens, x), 0, a.W - 1).T + bps - 1) / bps);
+    live = max(1, (key_plan(a, __builtin_amdgcn_readlane(lens, b), 0, a.W - 1).T + bps - 1) / bps);
   } else {
     const int group = r / a.grows;
     const int T = key_plan(a, a.seq_lens[b], a.by_G.quot(group * a.grows), a.by_G.quot(min(a.R, (group + 1) * a.grows) - 1)).T;
@@ -986,7 +969,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(SinkArgs a) {
 struct SinkPlan {
   bool tile;       // one tile of rows per workgroup, or blocks of rows
   int waves, tpw;  // block kernel
-  int groups, grows, nsplit, balanced, slots, unit;
+  int groups, grows, nsplit, balanced, slots;
 };
 static SinkPlan sink_plan(int B, int W, int nq, int nkv, int hd, int causal, int window, int sinks, int max_ctx) {
   SinkPlan s = {};
@@ -999,11 +982,10 @@ static SinkPlan sink_plan(int B, int W, int nq, int nkv, int hd, int causal, int
   }
   s.grows = s.tile ? 16 : s.waves * s.tpw * 16;
   s.groups = (int)ceil_div(R, s.grows);
-  s.unit = s.tile ? 4 * (hd == 128 ? kTileBlocks<128> : kTileBlocks<256>) : 4;  // a step of each wave; two chunks of 64 keys
   // blocks of 32 keys a pass may look at (the sliding window's rows, and its sinks)
   int64_t span = max_ctx;
   if (causal && window > 0) span = std::min<int64_t>(span, (int64_t)window + W + sinks + 96);
-  const int64_t most = std::max<int64_t>(1, ceil_div(ceil_div(span, 32) + 1, s.unit));
+  const int64_t most = std::max<int64_t>(1, ceil_div(ceil_div(span, 32) + 1, kSplitUnit));
   // workgroups that run at once: two per CU, one of the tile kernel at head_dim 256 (its registers)
   const int64_t tasks = (int64_t)B * nkv * s.groups, want = s.tile && hd == 256 ? 256 : 512;
   s.nsplit = (int)std::min<int64_t>(most, std::max<int64_t>(1, want / tasks));
@@ -1076,7 +1058,7 @@ extern "C" int dsk_attention_sinks(const uint16_t* q, int B, int W, int nq, int 
   DSK_REQUIRE(((uintptr_t)workspace & 15) == 0 || need == 0, "%s: workspace must be 16-byte aligned", who);
   SinkArgs a = {q, B, W, nq, nkv, nq / nkv, (int)R, scale, softcap, causal ? 1 : 0, window, sinks, seq_lens, block_table,
                 max_pages, page, k_pool, v_pool, k_sb, v_sb, out, out_packed ? 1 : 0, s.groups, s.grows, s.slots, s.nsplit,
-                s.balanced, s.unit, reinterpret_cast<float*>(workspace),
+                s.balanced, reinterpret_cast<float*>(workspace),
                 reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + sink_part_o_bytes(s, R, nkv, hd)),
                 FastDiv(page), FastDiv(nq / nkv), FastDiv(nkv), FastDiv(s.nsplit)};
 #define DSK_SINKS(HDV)                                                                                \
