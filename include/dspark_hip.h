@@ -339,8 +339,8 @@ int dsk_attention_rows(const uint16_t* q, int B, int W, int nq, int nkv, int hd,
  * (window 0: no window). Any number of new tokens per row: decode and verify passes split the keys over
  * the chip (a batch's rows by their lengths, read on the device) and join the splits in a second kernel;
  * prompts run in blocks of query rows. k and v of quantised caches are the values dsk_kv_read returns;
- * scores, softmax statistics and outputs stay float32, a probability enters P.V as two bf16 terms
- * (within 2^-17). What stands in a masked key, or in the slots behind the last one, never reaches the
+ * scores, softmax statistics and outputs stay float32, a probability enters P.V as p_terms bf16 terms: 3
+ * (within 2^-26), or for W > 64 also 2 (2^-17, as dsk_attention's many-query form). What stands in a masked key, or in the slots behind the last one, never reaches the
  * output, infinities and NaN included; a row that sees no key becomes zeros. softcap as dsk_attention.
  * head_dim 128 or 256, pages of a multiple of 32 tokens, scale > 0, 16-byte aligned buffers. max_ctx
  * bounds seq_lens[b] + W and sizes the grid (graph-stable). workspace:
@@ -349,8 +349,8 @@ int dsk_attention_rows(const uint16_t* q, int B, int W, int nq, int nkv, int hd,
 size_t dsk_attention_sinks_ws_bytes(int B, int W, int nq, int nkv, int hd, int causal, int window,
                                     int sinks, int max_ctx);
 int dsk_attention_sinks(const uint16_t* q, int B, int W, int nq, int nkv, int hd, float scale, int causal,
-                        int window, int sinks, float softcap, const int32_t* seq_lens, int max_ctx,
-                        const int32_t* block_table, int max_pages, int page, int kv_dtype,
+                        int window, int sinks, float softcap, int p_terms, const int32_t* seq_lens,
+                        int max_ctx, const int32_t* block_table, int max_pages, int page, int kv_dtype,
                         const void* k_pool, const void* v_pool, const uint32_t* k_sb,
                         const uint32_t* v_sb, uint16_t* out, int out_packed, void* workspace,
                         size_t ws_bytes, dsk_stream_t stream);

@@ -6,7 +6,9 @@
 // 16 + 4 g + r of a 32-key block, which are its 8 items of the P operand, and V^T comes in that key order.
 // Keys are visited in aligned blocks of 32: first the blocks that hold sinks, then those from the window's
 // start (or 0) to the last key. Scores, running maximum, sum and output are float32; a probability enters
-// the P.V product as two bf16 terms (within 2^-17 of it).
+// the P.V product as three bf16 terms (within 2^-26 of it), in passes of many rows also as two (2^-17), as the
+// caller says: two moved the logits of small models to twice the distance that float32 orders of summation
+// alone move them by, three left them there; they cost a prompt of 4096 rows 18 %, decoding 9 %.
 //
 // The maximum moves only when a score passes it by 2^8: below that the exponentials stay in float32's
 // range and nothing is lost, and a block costs one vote instead of two lane exchanges and a rescale.
@@ -55,6 +57,7 @@ struct SinkArgs {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kSplitUnit = 4;       // splits are multiples of this many 32-key blocks: one per wave, or two chunks of 64
 constexpr float kMaxSlack = 8.0f;   // how far (log2) a score may pass the running maximum
+constexpr int kDecodeMaxW = 64;      // new tokens per row of a decode or verify pass
 constexpr int kBalancedRows = 64;   // rows whose lengths a workgroup reads to place its split
 
 // The 32-key blocks that query tokens i0 .. i1 of row b look at.
@@ -172,8 +175,9 @@ __device__ __forceinline__ void static_for(F f) {
   }
 }
 
-// The running state of one tile of 16 queries over the keys seen so far.
-template <int HD>
+// The running state of one tile of 16 queries over the keys seen so far; a probability goes into the P.V
+// products as kTerms bf16 terms.
+template <int HD, int kTerms>
 struct Tile {
   float m, l;  // maximum (times c2) of the lane's query; the lane's own keys' sum
   f32x4 o[HD / 16];
@@ -208,38 +212,41 @@ struct Tile {
         l += st[t][r];
       }
   }
-  // the two bf16 terms of 8 probabilities (tiles t, t + 1 of a 32-key block)
-  static __device__ __forceinline__ void terms(const f32x4& a, const f32x4& b, u32x4& hi, u32x4& lo) {
-    uint32_t h[4], w[4];
-    split2_bf16x2(a[0], a[1], h[0], w[0]);
-    split2_bf16x2(a[2], a[3], h[1], w[1]);
-    split2_bf16x2(b[0], b[1], h[2], w[2]);
-    split2_bf16x2(b[2], b[3], h[3], w[3]);
-    hi = u32x4{h[0], h[1], h[2], h[3]};
-    lo = u32x4{w[0], w[1], w[2], w[3]};
+  // the bf16 terms of 8 probabilities (tiles t, t + 1 of a 32-key block)
+  static __device__ __forceinline__ void terms(const f32x4& a, const f32x4& b, u32x4 (&t)[kTerms]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4& s = i < 2 ? a : b;
+      uint32_t w[kTerms];
+      split_terms_bf16x2<kTerms>(s[2 * (i & 1)], s[2 * (i & 1) + 1], w);
+#pragma unroll
+      for (int k = 0; k < kTerms; ++k) t[k][i] = w[k];
+    }
   }
-  // O^T += V^T . P^T for d tiles D .. D + 3 and a block's 32 keys. The first terms of the four, then the
-  // second ones: four independent products between two on the same accumulator.
+  // O^T += V^T . P^T for d tiles D .. D + 3 and a block's 32 keys, term by term: four independent products
+  // between two on the same accumulator.
   template <int D>
-  __device__ __forceinline__ void add4(const u32x4 (&v)[4], u32x4 hi, u32x4 lo) {
+  __device__ __forceinline__ void add4(const u32x4 (&v)[4], const u32x4 (&t)[kTerms]) {
 #pragma unroll
-    for (int d = 0; d < 4; ++d) o[D + d] = mfma16(v[d], hi, o[D + d]);
+    for (int k = 0; k < kTerms; ++k)
 #pragma unroll
-    for (int d = 0; d < 4; ++d) o[D + d] = mfma16(v[d], lo, o[D + d]);
+      for (int d = 0; d < 4; ++d) o[D + d] = mfma16(v[d], t[k], o[D + d]);
   }
   // The infinities and NaN of those operands, where not every query sees every key: the products take the
   // operands without them (finite_only), and each is added here to the queries that see its key.
   // raw(d, k, g, r): the bf16 value of key k, dim 16 (D + d) + 4 g + r. Rare, and written to cost the common
   // path no registers.
   template <int D, class Raw>
-  __device__ __forceinline__ void add_nonfinite(const Sight& see, int base, int lane, u32x4 hi, u32x4 lo, Raw raw) {
+  __device__ __forceinline__ void add_nonfinite(const Sight& see, int base, int lane, const u32x4 (&t)[kTerms], Raw raw) {
 #pragma unroll 1
     for (int k = 0; k < 32; ++k) {
       const int e = (k / 16) * 4 + k % 4, from = (lane & 15) + 16 * ((k % 16) / 4);
-      const uint32_t h = e < 4 ? (e < 2 ? hi[0] : hi[1]) : (e < 6 ? hi[2] : hi[3]);
-      const uint32_t w = e < 4 ? (e < 2 ? lo[0] : lo[1]) : (e < 6 ? lo[2] : lo[3]);
-      const int sh = e & 1 ? 0 : 16;
-      float p = bits_f32((h << sh) & 0xffff0000u) + bits_f32((w << sh) & 0xffff0000u);
+      float p = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kTerms; ++i) {
+        const uint32_t w = e < 4 ? (e < 2 ? t[i][0] : t[i][1]) : (e < 6 ? t[i][2] : t[i][3]);
+        p += bits_f32((w << (e & 1 ? 0 : 16)) & 0xffff0000u);
+      }
       p = __shfl(p, from, 64);
       const bool vis = see.sees(base + k);
 #pragma unroll
@@ -545,7 +552,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ?
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(src + KRaw<HD, KVT>::dim(s, g));
   }
-  Tile<HD> tile;
+  Tile<HD, 3> tile;
   tile.clear();
   uint8_t* vlds = lds + wv * DT * kVTile;
   if (nblk > 0) {  // the loop within: around it, the count of loads in flight would have to hold for no loads too
@@ -577,8 +584,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ?
       }
       if (!open) mask_scores(see, st, 0, base, g);
       tile.soften(st, c2);
-      u32x4 hi, lo;
-      Tile<HD>::terms(st[0], st[1], hi, lo);
+      u32x4 pt[3];
+      Tile<HD, 3>::terms(st[0], st[1], pt);
       if constexpr (kRows) {
 #pragma unroll
         for (int u = 0; u < NI; ++u) {
@@ -600,7 +607,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ?
           v4.operands(Q, y);
         }
         if (!open && any_nonfinite(y)) {
-          tile.template add_nonfinite<D>(see, base, lane, hi, lo, [&](int d, int k, int gg, int rr) -> uint32_t {
+          tile.template add_nonfinite<D>(see, base, lane, pt, [&](int d, int k, int gg, int rr) -> uint32_t {
             const int e = (k / 16) * 4 + k % 4, at = 4 * gg + rr + 16 * ((k % 16) / 4);  // the lane that holds it
             if constexpr (kRows) {
               return *reinterpret_cast<const uint16_t*>(vlds + (D + d) * kVTile + (at >> 4) * kVGroup + (at & 15) * 16 + 2 * e);
@@ -613,7 +620,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ?
 #pragma unroll
           for (int d = 0; d < 4; ++d) y[d] = finite_only(y[d]);
         }
-        tile.template add4<D>(y, hi, lo);
+        tile.template add4<D>(y, pt);
       });
       if constexpr (kRows) asm volatile("" ::: "memory");
       load_v(tok_nx);
@@ -666,7 +673,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ?
 // are 64 keys at head_dim 128 and 32 at 256, so a buffer is 33 KB: two workgroups of four waves fit a CU.
 template <int HD> constexpr int kChunkBlocks = HD == 128 ? 2 : 1;
 
-template <int HD, int KVT, int NW, int TPW>
+template <int HD, int KVT, int NW, int TPW, int TERMS>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_block_kernel(SinkArgs a) {
   constexpr int KS = HD / 32, DT = HD / 16, NB = kChunkBlocks<HD>, NKT = 2 * NB;
   constexpr bool kRows = KVT != DSK_KV_U4;
@@ -776,7 +783,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     }
   };
 
-  Tile<HD> tile[TPW];
+  Tile<HD, TERMS> tile[TPW];
 #pragma unroll
   for (int u = 0; u < TPW; ++u) tile[u].clear();
 
@@ -804,7 +811,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
         for (int u = 0; u < TPW; ++u) st[u][x] = mfma16(kf, qf[u][s], st[u][x]);
       }
-    u32x4 hi[TPW][NB], lo[TPW][NB];
+    u32x4 pt[TPW][NB][TERMS];
 #pragma unroll
     for (int u = 0; u < TPW; ++u) {
       if (a.softcap > 0.0f) {
@@ -819,7 +826,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       }
       tile[u].soften(st[u], c2);
 #pragma unroll
-      for (int x = 0; x < NB; ++x) Tile<HD>::terms(st[u][2 * x], st[u][2 * x + 1], hi[u][x], lo[u][x]);
+      for (int x = 0; x < NB; ++x) Tile<HD, TERMS>::terms(st[u][2 * x], st[u][2 * x + 1], pt[u][x]);
     }
 #pragma unroll
     for (int x = 0; x < NB; ++x) {
@@ -832,7 +839,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         if (!open && any_nonfinite(w)) {
 #pragma unroll
           for (int u = 0; u < TPW; ++u)
-            tile[u].template add_nonfinite<D>(see[u], base[x], lane, hi[u][x], lo[u][x], [&](int d, int k, int gg, int rr) -> uint32_t {
+            tile[u].template add_nonfinite<D>(see[u], base[x], lane, pt[u][x], [&](int d, int k, int gg, int rr) -> uint32_t {
               return *reinterpret_cast<const uint16_t*>(vb8 + (D + d) * kVTile + ((k % 16) / 4) * kVGroup + (4 * gg + rr) * 16 +
                                                         2 * ((k / 16) * 4 + k % 4));
             });
@@ -840,7 +847,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
           for (int d = 0; d < 4; ++d) w[d] = finite_only(w[d]);
         }
 #pragma unroll
-        for (int u = 0; u < TPW; ++u) tile[u].template add4<D>(w, hi[u][x], lo[u][x]);
+        for (int u = 0; u < TPW; ++u) tile[u].template add4<D>(w, pt[u][x]);
       });
     }
   };
@@ -1001,14 +1008,19 @@ static size_t sink_ws(const SinkPlan& s, int64_t R, int nkv, int hd) {
 }
 
 template <int HD, int KVT>
-static void launch_sinks(const SinkArgs& a, const SinkPlan& s, hipStream_t st) {
+static void launch_sinks(const SinkArgs& a, const SinkPlan& s, int terms, hipStream_t st) {
   const dim3 grid((unsigned)(s.slots * a.nkv), (unsigned)s.groups);
   if (s.tile) {
     hipLaunchKernelGGL((attention_tile_kernel<HD, KVT>), grid, dim3(256), 0, st, a);
   } else if (s.waves == 8) {
-    if constexpr (HD == 128) hipLaunchKernelGGL((attention_block_kernel<HD, KVT, 8, 2>), grid, dim3(512), 0, st, a);
+    if constexpr (HD == 128) {
+      if (terms == 2) hipLaunchKernelGGL((attention_block_kernel<HD, KVT, 8, 2, 2>), grid, dim3(512), 0, st, a);
+      else hipLaunchKernelGGL((attention_block_kernel<HD, KVT, 8, 2, 3>), grid, dim3(512), 0, st, a);
+    }
+  } else if (terms == 2) {
+    hipLaunchKernelGGL((attention_block_kernel<HD, KVT, 4, 1, 2>), grid, dim3(256), 0, st, a);
   } else {
-    hipLaunchKernelGGL((attention_block_kernel<HD, KVT, 4, 1>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attention_block_kernel<HD, KVT, 4, 1, 3>), grid, dim3(256), 0, st, a);
   }
   if (s.nsplit > 1)
     hipLaunchKernelGGL((attention_join_kernel<HD>), dim3((unsigned)a.R, (unsigned)(a.B * a.nkv)), dim3(256), 0, st, a);
@@ -1026,8 +1038,8 @@ extern "C" size_t dsk_attention_sinks_ws_bytes(int B, int W, int nq, int nkv, in
 }
 
 extern "C" int dsk_attention_sinks(const uint16_t* q, int B, int W, int nq, int nkv, int hd, float scale, int causal,
-                                   int window, int sinks, float softcap, const int32_t* seq_lens, int max_ctx,
-                                   const int32_t* block_table, int max_pages, int page, int kv_dtype,
+                                   int window, int sinks, float softcap, int p_terms, const int32_t* seq_lens,
+                                   int max_ctx, const int32_t* block_table, int max_pages, int page, int kv_dtype,
                                    const void* k_pool, const void* v_pool, const uint32_t* k_sb, const uint32_t* v_sb,
                                    uint16_t* out, int out_packed, void* workspace, size_t ws_bytes,
                                    dsk_stream_t stream) {
@@ -1036,6 +1048,8 @@ extern "C" int dsk_attention_sinks(const uint16_t* q, int B, int W, int nq, int 
   DSK_REQUIRE(hd == 128 || hd == 256, "%s: head_dim %d not supported (128, 256)", who, hd);
   DSK_REQUIRE(B > 0 && W > 0 && nq > 0 && nkv > 0 && nq % nkv == 0, "%s: bad shape", who);
   DSK_REQUIRE(scale > 0.0f && softcap >= 0.0f, "%s: scale must be positive, softcap not negative", who);
+  DSK_REQUIRE(p_terms == 3 || (p_terms == 2 && W > kDecodeMaxW), "%s: %d terms of a probability (3; 2 for more than %d new "
+              "tokens)", who, p_terms, kDecodeMaxW);
   DSK_REQUIRE(window >= 0 && sinks >= 0 && window < 0x20000000 && sinks < 0x20000000, "%s: window %d, sinks %d", who, window, sinks);
   DSK_REQUIRE(kv_dtype == DSK_KV_BF16 || kv_dtype == DSK_KV_U8 || kv_dtype == DSK_KV_U4, "%s: kv_dtype %d", who, kv_dtype);
   DSK_REQUIRE(kv_dtype == DSK_KV_BF16 || (k_sb && v_sb), "%s: quantised KV needs scale/bias buffers", who);
@@ -1062,9 +1076,9 @@ extern "C" int dsk_attention_sinks(const uint16_t* q, int B, int W, int nq, int 
                 reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + sink_part_o_bytes(s, R, nkv, hd)),
                 FastDiv(page), FastDiv(nq / nkv), FastDiv(nkv), FastDiv(s.nsplit)};
 #define DSK_SINKS(HDV)                                                                                \
-  if (kv_dtype == DSK_KV_BF16) launch_sinks<HDV, DSK_KV_BF16>(a, s, as_stream(stream));               \
-  else if (kv_dtype == DSK_KV_U8) launch_sinks<HDV, DSK_KV_U8>(a, s, as_stream(stream));              \
-  else launch_sinks<HDV, DSK_KV_U4>(a, s, as_stream(stream))
+  if (kv_dtype == DSK_KV_BF16) launch_sinks<HDV, DSK_KV_BF16>(a, s, p_terms, as_stream(stream));      \
+  else if (kv_dtype == DSK_KV_U8) launch_sinks<HDV, DSK_KV_U8>(a, s, p_terms, as_stream(stream));     \
+  else launch_sinks<HDV, DSK_KV_U4>(a, s, p_terms, as_stream(stream))
   if (hd == 128) {
     DSK_SINKS(128);
   } else {

@@ -524,29 +524,40 @@ def _sinks_ws_bytes(*args) -> int:
     return _hip.lib.dsk_attention_sinks_ws_bytes(*args)
 
 
+def _attention_sinks(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table, page, kv_dtype, k_pool, v_pool, k_sb,
+                     v_sb, causal, window, softcap, sinks, out, p_terms):
+    """dsk_attention_sinks into out (bf16 rows or a Packed)."""
+    _on_device(q)
+    packed = isinstance(out, Packed)
+    odata = out.data if packed else out
+    if q.dtype != torch.bfloat16 or not q.is_contiguous() or q.numel() != B * W * nq * hd:
+        raise ValueError(f"attention: q must be contiguous bf16 [{B * W}, {nq * hd}]")
+    if odata.dtype != torch.bfloat16 or not odata.is_contiguous() or (not packed and odata.numel() != q.numel()):
+        raise ValueError(f"attention: out must be contiguous bf16 [{B * W}, {nq * hd}]")
+    if seq_lens.dtype != torch.int32 or seq_lens.numel() != B or block_table.dtype != torch.int32 or \
+            block_table.shape[0] != B or not (seq_lens.is_contiguous() and block_table.is_contiguous()):
+        raise ValueError(f"attention: seq_lens and block_table must be contiguous int32 of {B} rows")
+    args = (B, W, nq, nkv, hd, int(bool(causal)), int(window), int(sinks), int(max_ctx))
+    need = _sinks_ws_bytes(*args)
+    # per call: passes on two streams, or of two captured graphs, may overlap
+    buf = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    call("dsk_attention_sinks", addr(q), *args[:5], scale, *args[5:8], softcap, p_terms, addr(seq_lens), args[8],
+         addr(block_table), block_table.shape[1], page, kv_dtype, addr(k_pool), addr(v_pool), addr(k_sb), addr(v_sb),
+         addr(odata), int(packed), addr(buf), need, stream_ptr())
+
+
 def attention(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table, page, kv_dtype, k_pool,
               v_pool, k_sb=None, v_sb=None, *, causal=True, window=0, softcap=0.0, out=None, packed=False, sinks=0):
     """Returns bf16 [B*W, nq*hd], or a Packed [B*W, nq*hd] (the o-projection's x) when packed. sinks: the
     context's first tokens that stay visible beside a sliding window (causal). 4-bit caches and sinks run
-    dsk_attention_sinks, which takes any W."""
+    dsk_attention_sinks, which takes any W (probabilities as two bf16 terms past 64, as here without them)."""
     if out is None:
         out = Packed.empty(B * W, nq * hd, q.device) if packed else torch.empty(
             (B * W, nq * hd), dtype=torch.bfloat16, device=q.device)
     odata = out.data if isinstance(out, Packed) else out
     if sinks or kv_dtype == DSK_KV_U4:
-        _on_device(q)
-        if q.dtype != torch.bfloat16 or not q.is_contiguous() or q.numel() != B * W * nq * hd:
-            raise ValueError(f"attention: q must be contiguous bf16 [{B * W}, {nq * hd}]")
-        if odata.dtype != torch.bfloat16 or not odata.is_contiguous() or (
-                not isinstance(out, Packed) and odata.numel() != B * W * nq * hd):
-            raise ValueError(f"attention: out must be contiguous bf16 [{B * W}, {nq * hd}]")
-        args = (B, W, nq, nkv, hd, int(bool(causal)), int(window), int(sinks), int(max_ctx))
-        need = _sinks_ws_bytes(*args)
-        # per call: passes on two streams, or of two captured graphs, may overlap
-        buf = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        call("dsk_attention_sinks", addr(q), *args[:5], scale, *args[5:8], softcap, addr(seq_lens), args[8],
-             addr(block_table), block_table.shape[1], page, kv_dtype, addr(k_pool), addr(v_pool), addr(k_sb),
-             addr(v_sb), addr(odata), int(isinstance(out, Packed)), addr(buf), need, stream_ptr())
+        _attention_sinks(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table, page, kv_dtype, k_pool, v_pool,
+                         k_sb, v_sb, causal, window, softcap, sinks, out, 2 if W > 64 else 3)
         return out
     ws = Workspace.get(q.device)
     need = _hip.lib.dsk_attn_ws_bytes(B, W, nq, hd, max_ctx)
@@ -590,9 +601,14 @@ def attention_rows(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table, 
     probabilities (dsk_attention_rows; dsk_attention where its shapes end, with scratch for every row and
     key split: by attention_rows_takes a caller can give that one fewer rows at a time). 4-bit caches and
     sinks: as attention."""
-    if sinks or kv_dtype == DSK_KV_U4 or not attention_rows_takes(hd, block_table.shape[1]):
+    if sinks or kv_dtype == DSK_KV_U4:
+        out = torch.empty((B * W, nq * hd), dtype=torch.bfloat16, device=q.device)
+        _attention_sinks(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table, page, kv_dtype, k_pool, v_pool,
+                         k_sb, v_sb, causal, window, 0.0, sinks, out, 3)
+        return out
+    if not attention_rows_takes(hd, block_table.shape[1]):
         return attention(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table, page, kv_dtype, k_pool, v_pool,
-                         k_sb, v_sb, causal=causal, window=window, sinks=sinks)
+                         k_sb, v_sb, causal=causal, window=window)
     out = torch.empty((B * W, nq * hd), dtype=torch.bfloat16, device=q.device)
     call("dsk_attention_rows", ptr(q), B, W, nq, nkv, hd, float(scale), int(bool(causal)), int(window), ptr(seq_lens),
          ptr(block_table), block_table.shape[1], page, kv_dtype, ptr(k_pool), ptr(v_pool), ptr(k_sb), ptr(v_sb),

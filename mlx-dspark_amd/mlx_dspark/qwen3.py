@@ -63,6 +63,7 @@ class TargetArgs:
     final_logit_softcapping: float | None = None
     query_pre_attn_scalar: float | None = None    # attention scale = this ** -0.5 when set
     rope_local_base_freq: float | None = None     # RoPE base of the sliding-window layers
+    attention_sinks: int = 0                       # first tokens the sliding-window layers keep seeing
 
     @property
     def sandwich_norms(self) -> bool:
@@ -84,6 +85,9 @@ class TargetArgs:
         if self.is_sliding(layer) and self.sliding_window:
             return int(self.sliding_window)
         return 0
+
+    def sinks(self, layer: int) -> int:
+        return int(self.attention_sinks) if self.window(layer) else 0
 
 
 @dataclass
@@ -182,7 +186,7 @@ class Qwen3W8:
                                 k_pool, v_pool, k_sb, v_sb, x=x)
         o = ops.attention(q, B, W, nq, nkv, hd, a.attn_scale, cache.seq_lens, cache.max_ctx,
                           cache.block_table, cache.page, cache.kv_dtype, k_pool, v_pool, k_sb, v_sb,
-                          causal=causal, window=a.window(l), packed=True)
+                          causal=causal, window=a.window(l), packed=True, sinks=a.sinks(l))
         if not a.sandwich_norms:
             # the residual adds run in the o / down epilogues, each next RMSNorm in the GEMM that
             # consumes it (normed later)
@@ -351,7 +355,7 @@ class Qwen3W8:
     def _rows_piece(self, cache: PagedKVCache) -> int:
         """Rows of one _rows_pass over this cache."""
         takes = ops.attention_rows_takes(self.args.head_dim, cache.block_table.shape[1])
-        return PREFILL_CHUNK if takes else SPLIT_CHUNK
+        return PREFILL_CHUNK if takes or cache.kv_dtype == ops.DSK_KV_U4 else SPLIT_CHUNK
 
     def _rows_attention(self, q: torch.Tensor, L: int, window: int, cache: PagedKVCache, l: int,
                         starts: list) -> torch.Tensor:
@@ -359,12 +363,15 @@ class Qwen3W8:
         or, after a long context, with key splits a few rows at a time."""
         a = self.args
         nq, nkv, hd = a.num_attention_heads, a.num_key_value_heads, a.head_dim
-        per = 0
-        if ops.attention_rows_takes(hd, cache.block_table.shape[1]):
+        per, sinks = 0, a.sinks(l)
+        whole = sinks > 0 or cache.kv_dtype == ops.DSK_KV_U4   # splits its keys by itself
+        if not whole and ops.attention_rows_takes(hd, cache.block_table.shape[1]):
             per = ops.attention_rows_split(L, nq, nkv, hd, cache.lengths[0], cache.max_ctx, window)
-        pools = (cache.max_ctx, cache.block_table, cache.page, cache.kv_dtype, *cache.layer_args(l))
+        ctx = cache.lengths[0] + L if whole else cache.max_ctx
+        pools = (ctx, cache.block_table, cache.page, cache.kv_dtype, *cache.layer_args(l))
         if per == 0:
-            return ops.attention_rows(q, 1, L, nq, nkv, hd, a.attn_scale, cache.seq_lens, *pools, window=window)
+            return ops.attention_rows(q, 1, L, nq, nkv, hd, a.attn_scale, cache.seq_lens, *pools, window=window,
+                                      sinks=sinks)
         if not starts:
             starts.extend(cache.seq_lens + r for r in range(0, L, per))
         out = torch.empty((L, nq * hd), dtype=torch.bfloat16, device=q.device)
@@ -475,6 +482,7 @@ class Qwen3W8:
         # the many-query kernel takes max_ctx as a bound of the keys only to choose its blocks; the split
         # ones (up to MAX_ROWS rows, other head_dims, very long caches) size their splits by it
         many = L > MAX_ROWS and hd == 128 and ops.attention_rows_takes(hd, cache.block_table.shape[1])
+        many = many or cache.kv_dtype == ops.DSK_KV_U4
         ctx = cache.lengths[0] + L if many else cache.max_ctx
         for l, Lw in enumerate(self.layers):
             ops.rows_rmsnorm(h, Lw.in_norm, eps, out=x)
@@ -484,7 +492,8 @@ class Qwen3W8:
             q = ops.qkv_rope_append(qkv, 1, L, nq, nkv, hd, Lw.q_norm, Lw.k_norm, eps, inv_freq, cache.seq_lens,
                                     cache.block_table, cache.page, cache.kv_dtype, k_pool, v_pool, k_sb, v_sb)
             o = ops.attention(q, 1, L, nq, nkv, hd, a.attn_scale, cache.seq_lens, ctx, cache.block_table,
-                              cache.page, cache.kv_dtype, k_pool, v_pool, k_sb, v_sb, causal=True, window=a.window(l))
+                              cache.page, cache.kv_dtype, k_pool, v_pool, k_sb, v_sb, causal=True, window=a.window(l),
+                              sinks=a.sinks(l))
             h.addmm_(o, rows(l, "o").t())
             ops.rows_rmsnorm(h, Lw.post_norm, eps, out=x)
             torch.matmul(x, rows(l, "gate_up").t(), out=gu)

@@ -28,8 +28,8 @@ class Target:
         self.is_vlm = False
         mt = getattr(model.args, "model_type", "qwen3")
         self.family = "gemma4" if mt.startswith("gemma") else mt
-        if kv_bits not in (None, 8):
-            raise ValueError(f"kv_bits={kv_bits}: the engine supports 8-bit KV (or bf16)")
+        if kv_bits not in (None, 4, 8):
+            raise ValueError(f"kv_bits={kv_bits}: the engine supports 8-bit and 4-bit KV (or bf16)")
         if kv_group_size != 64:
             raise ValueError("KV quantization uses group size 64")
         self.kv_bits = int(kv_bits) if kv_bits else None

@@ -227,14 +227,14 @@ def sdpa(q, K, V, scale, mask=None, p_bf16=False, *, split=0, block=0, partial_b
     return out.float()
 
 
-def causal_mask(offset: int, W: int, window: int = 0) -> torch.Tensor:
+def causal_mask(offset: int, W: int, window: int = 0, sinks: int = 0) -> torch.Tensor:
     """[W, offset + W] boolean: query i (absolute offset + i) sees key j iff j <= offset + i,
-    and, for a sliding-window layer, j > offset + i - window."""
+    and, for a sliding-window layer, j > offset + i - window or j < sinks."""
     j = torch.arange(offset + W)[None, :]
     i = torch.arange(W)[:, None]
     m = j <= offset + i
     if window:
-        m &= j > offset + i - window
+        m &= (j > offset + i - window) | (j < sinks)
     return m
 
 
@@ -264,11 +264,11 @@ def deq_table(t) -> torch.Tensor:
     return deq_codes(t.q, t.s, t.b)
 
 
-def kv_quant_roundtrip(x: torch.Tensor) -> torch.Tensor:
-    """8-bit group-64 affine round trip along the last axis (same rule as the weights)."""
+def kv_quant_roundtrip(x: torch.Tensor, bits: int = 8) -> torch.Tensor:
+    """8-bit (4-bit) group-64 affine round trip along the last axis (same rule as the weights)."""
     shp = x.shape
     flat = x.reshape(-1, shp[-1]).numpy().astype(np.float32)
-    q, s, b = W8.quantize(flat)
+    q, s, b = W8.quantize(flat, bits)
     return bf(torch.from_numpy(W8.dequantize(q, s, b).astype(np.float32)).reshape(shp))
 
 
@@ -322,6 +322,14 @@ class OracleTarget:
         # projections multiply weights rounded to bf16, as a bf16 library GEMM over expanded
         # weights does); the final norm and head keep the engine's normed-later form
         self.dense = False
+        # a 4-bit cache quantises float32 rows: those of the projection's float32 sums, or (True: the
+        # engine's passes of many rows) of its bf16 output
+        self.proj_bf16 = False
+        # given: per layer (K, V) of all positions up to the forward's last, used in place of the oracle's own
+        # cache (an engine's cache read back: a quantised code that two evaluations round apart is a step of
+        # its group's range, which would travel on); rows: per layer the forward's K, V before they are cached
+        self.given = None
+        self.rows: dict = {}
         self._bf_w: dict = {}
 
     def _w(self, l: int, name: str) -> torch.Tensor:
@@ -356,22 +364,28 @@ class OracleTarget:
         for l, L in enumerate(self.layers):
             win = a.window(l)
             theta = (a.rope_local_base_freq or a.rope_theta) if a.is_sliding(l) else a.rope_theta
+            kv4 = self.kv_bits == 4
+            proj = (lambda x: x) if kv4 and not (self.proj_bf16 or self.dense) else bf
             if first:
-                qkv = bf(mm(bf(rmsnorm(h, L.in_norm, eps)), self._w(l, "wq")))
+                qkv = proj(mm(bf(rmsnorm(h, L.in_norm, eps)), self._w(l, "wq")))
             else:
                 xg, r = norm_later(h, L.in_norm, eps)
-                qkv = bf(r * mm(xg, L.wq))
+                qkv = proj(r * mm(xg, L.wq))
             q = qkv[:, : nq * hd].view(W, nq, hd)
             k = qkv[:, nq * hd:(nq + nkv) * hd].view(W, nkv, hd)
             v = qkv[:, (nq + nkv) * hd:].view(W, nkv, hd)
-            q = bf(rope(bf(rmsnorm(q, L.q_norm, eps)).transpose(0, 1), pos, theta, revolutions=rev).transpose(0, 1))
-            k = bf(rope(bf(rmsnorm(k, L.k_norm, eps)).transpose(0, 1), pos, theta, revolutions=rev).transpose(0, 1))
-            if self.kv_bits == 8 and self.requant_new:
-                k, v = kv_quant_roundtrip(k), kv_quant_roundtrip(v)
+            rnd = (lambda x: x) if kv4 else bf
+            q = bf(rope(rnd(rmsnorm(q, L.q_norm, eps)).transpose(0, 1), pos, theta, revolutions=rev).transpose(0, 1))
+            k = rnd(rope(rnd(rmsnorm(k, L.k_norm, eps)).transpose(0, 1), pos, theta, revolutions=rev).transpose(0, 1))
+            self.rows[l] = (k, v)
+            if kv4 or (self.kv_bits == 8 and self.requant_new):
+                k, v = kv_quant_roundtrip(k, self.kv_bits), kv_quant_roundtrip(v, self.kv_bits)
             self.K[l] = torch.cat([self.K[l], k])
             self.V[l] = torch.cat([self.V[l], v])
-            o = bf(sdpa(q, self.K[l], self.V[l], a.attn_scale, causal_mask(self.offset, W, win), self.p_bf16,
-                        **self.attn_opts))
+            if self.given is not None:
+                self.K[l], self.V[l] = self.given[l]
+            o = bf(sdpa(q, self.K[l], self.V[l], a.attn_scale, causal_mask(self.offset, W, win, a.sinks(l)),
+                        self.p_bf16, **self.attn_opts))
             if L.attn_out_norm is not None:     # sandwich: norm the projection output, then add
                 h = bf(h + bf(rmsnorm(bf(mm(o.reshape(W, -1), L.wo)), L.attn_out_norm, eps)))
             else:

@@ -79,7 +79,7 @@ def visible(n, W, total, causal, window, sinks):
 
 
 def reference(cache, q, lens, W, nq, nkv, causal, window, sinks, scale, softcap=0.0):
-    """(out, tolerance) float64 [B, W, nq, hd]. A probability is off by its two bf16 terms (2^-17), by the
+    """(out, tolerance) float64 [B, W, nq, hd]. A probability is off by its bf16 terms (two: 2^-17), by the
     float32 error of its score (each of hd products and sums 2^-24 of the sum of magnitudes, twice: in the
     score and in the maximum) and by its sum's (n additions); the result by one bf16 rounding."""
     B, hd, G = len(lens), cache.hd, nq // nkv
@@ -163,12 +163,10 @@ CASES = [
 ]
 
 
-@pytest.mark.parametrize("bits", [4, 8, 0])
-@pytest.mark.parametrize("case", CASES, ids=str)
+# without sinks the other cache types run kernels of their own
+@pytest.mark.parametrize("case,bits", [(c, bits) for c in CASES for bits in (4, 8, 0) if bits == 4 or c[-1]], ids=str)
 def test_attention(dev, case, bits):
     hd, nq, nkv, page, W, lens, causal, window, sinks = case
-    if bits != 4 and not sinks:
-        pytest.skip("the other cache types' kernels")
     print(f"attention bits={bits} {case}", flush=True)
     max_pages = -(-(max(lens) + W) // page) + 1
     c = Cache(bits, len(lens), nkv, hd, max_pages, page, seed=W + hd)
@@ -204,6 +202,7 @@ def test_softcap_scale_and_sharp_scores(dev, W, nq, nkv, hd):
     """Soft-capped scores, another scale, and scores so large that the maximum moves block after block."""
     c = Cache(4, 1, nkv, hd, 12, 64, seed=3)
     q = queries(1, W, nq, hd, 2, std=8.0)
+    # past 64 new tokens ops.attention takes the form with two terms of a probability
     for scale, cap in ((1.0, 30.0), (0.37, 0.0)):
         want, tol = reference(c, q, [600], W, nq, nkv, True, 0, 0, scale, cap)
         # tanh's argument and value: a few float32 roundings of a score of up to `cap`

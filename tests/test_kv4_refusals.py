@@ -54,7 +54,7 @@ def test_cache_refuses():
 
 def _attend(**kw):
     from mlx_dspark import _hip
-    a = dict(q=P, B=1, W=1, nq=4, nkv=2, hd=128, scale=0.1, causal=1, window=0, sinks=0, cap=0.0, sl=P, max_ctx=100,
+    a = dict(q=P, B=1, W=1, nq=4, nkv=2, hd=128, scale=0.1, causal=1, window=0, sinks=0, cap=0.0, terms=3, sl=P, max_ctx=100,
              table=P, max_pages=2, page=64, kv=2, k=P, v=P, ks=P, vs=P, out=P, packed=0, ws=None, wsb=0, st=None)
     a.update(kw)
     return _hip.lib.dsk_attention_sinks(*a.values()), _hip.lib.dsk_last_error().decode()
@@ -66,7 +66,7 @@ def _attend(**kw):
     (dict(sinks=-1), "sinks"), (dict(kv=3), "kv_dtype"), (dict(ks=None), "scale/bias"), (dict(kv=0, page=48), "multiples of 32"),
     (dict(page=16), "multiples of 32"), (dict(max_ctx=129), "max_ctx"), (dict(W=2, max_ctx=1), "max_ctx"),
     (dict(out=ctypes.c_void_p((1 << 20) + 8)), "aligned"), (dict(W=65, packed=1), "packed"),
-    (dict(max_pages=1 << 24), "block table"),
+    (dict(max_pages=1 << 24), "block table"), (dict(terms=2), "terms"), (dict(terms=1, W=90), "terms"),
 ])
 def test_attention_refuses(kw, word):
     rc, msg = _attend(**kw)
