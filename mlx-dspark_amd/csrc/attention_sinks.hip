@@ -161,6 +161,10 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 __device__ __forceinline__ bool nonfinite2(uint32_t w) {
   return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
+// whether 4-bit values under this scale and offset may pass the largest float (the others do not, in 32 bits)
+__device__ __forceinline__ bool wide2(uint32_t sb) {
+  return (sb & 0x7f80u) >= 0x7d00u || (sb & 0x7f800000u) >= 0x7d000000u;  // 2^123 or more: 15 s + |b| < 2^127 below
+}
 __device__ __forceinline__ int64_t sink_out_index(const SinkArgs& a, int HD, int b, int r, int kvh, int d) {
   const int i = a.by_G.quot(r);
   const int64_t m = (int64_t)b * a.W + i, k = (int64_t)(kvh * a.G + r - i * a.G) * HD + d;
@@ -187,30 +191,39 @@ struct Tile {
 #pragma unroll
     for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0, 0, 0, 0};
   }
-  // scores -> probabilities in place
+  // the lane's largest score (times c2)
   template <int NKT>
-  __device__ __forceinline__ void soften(f32x4 (&st)[NKT], float c2) {
+  static __device__ __forceinline__ float largest(const f32x4 (&st)[NKT], float c2) {
     float mx = -__builtin_inff();
 #pragma unroll
     for (int t = 0; t < NKT; ++t) mx = fmaxf(mx, fmaxf(fmaxf(st[t][0], st[t][1]), fmaxf(st[t][2], st[t][3])));
-    if (__any(mx * c2 > m + kMaxSlack)) {
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float mn = fmaxf(m, mx * c2);
-      const float alpha = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= alpha;
+    return mx * c2;
+  }
+  // whether a score passes the running maximum by more than its slack; if so for any lane, raise() in all
+  __device__ __forceinline__ bool passes(float mx) const { return mx > m + kMaxSlack; }
+  __device__ __forceinline__ void raise(float mx) {
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float mn = fmaxf(m, mx);
+    const float alpha = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= alpha;
 #pragma unroll
-      for (int d = 0; d < HD / 16; ++d) o[d] *= alpha;
-    }
+    for (int d = 0; d < HD / 16; ++d) o[d] *= alpha;
+  }
+  // a block's scores -> probabilities in place
+  __device__ __forceinline__ void soften(f32x4& a, f32x4& b, float c2) {
     const float mb = m == -__builtin_inff() ? 0.0f : m;  // a row with no visible key yet: exp2(-inf) = 0
 #pragma unroll
-    for (int t = 0; t < NKT; ++t)
+    for (int r = 0; r < 4; ++r) {
+      a[r] = __builtin_amdgcn_exp2f(fmaf(a[r], c2, -mb));
+      l += a[r];
+    }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        st[t][r] = __builtin_amdgcn_exp2f(fmaf(st[t][r], c2, -mb));
-        l += st[t][r];
-      }
+    for (int r = 0; r < 4; ++r) {
+      b[r] = __builtin_amdgcn_exp2f(fmaf(b[r], c2, -mb));
+      l += b[r];
+    }
   }
   // the bf16 terms of 8 probabilities (tiles t, t + 1 of a 32-key block)
   static __device__ __forceinline__ void terms(const f32x4& a, const f32x4& b, u32x4 (&t)[kTerms]) {
@@ -232,42 +245,7 @@ struct Tile {
 #pragma unroll
       for (int d = 0; d < 4; ++d) o[D + d] = mfma16(v[d], t[k], o[D + d]);
   }
-  // The infinities and NaN of those operands, where not every query sees every key: the products take the
-  // operands without them (finite_only), and each is added here to the queries that see its key.
-  // raw(d, k, g, r): the bf16 value of key k, dim 16 (D + d) + 4 g + r. Rare, and written to cost the common
-  // path no registers.
-  template <int D, class Raw>
-  __device__ __forceinline__ void add_nonfinite(const Sight& see, int base, int lane, const u32x4 (&t)[kTerms], Raw raw) {
-#pragma unroll 1
-    for (int k = 0; k < 32; ++k) {
-      const int e = (k / 16) * 4 + k % 4, from = (lane & 15) + 16 * ((k % 16) / 4);
-      float p = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kTerms; ++i) {
-        const uint32_t w = e < 4 ? (e < 2 ? t[i][0] : t[i][1]) : (e < 6 ? t[i][2] : t[i][3]);
-        p += bits_f32((w << (e & 1 ? 0 : 16)) & 0xffff0000u);
-      }
-      p = __shfl(p, from, 64);
-      const bool vis = see.sees(base + k);
-#pragma unroll
-      for (int d = 0; d < 4; ++d)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint32_t v = raw(d, k, lane >> 4, r);
-          const bool add = bool((int)((v & 0x7f80u) == 0x7f80u) & (int)vis);
-          o[D + d][r] = add ? fmaf(p, bits_f32(v << 16), o[D + d][r]) : o[D + d][r];
-        }
-    }
-  }
 };
-__device__ __forceinline__ bool any_nonfinite(const u32x4 (&v)[4]) {
-  bool bad = false;
-#pragma unroll
-  for (int d = 0; d < 4; ++d)
-#pragma unroll
-    for (int w = 0; w < 4; ++w) bad |= nonfinite2(v[d][w]);
-  return __any(bad);
-}
 __device__ __forceinline__ u32x4 finite_only(u32x4 x) {
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
@@ -275,6 +253,62 @@ __device__ __forceinline__ u32x4 finite_only(u32x4 x) {
     x[w] &= l | h;
   }
   return x;
+}
+// the value (bf16) of dim d of V at pool token tok; apart: whether it is staged as 0
+template <int HD, int KVT>
+__device__ __forceinline__ uint32_t v_value(const SinkArgs& a, uint32_t tok, int d, bool& apart) {
+  if constexpr (KVT == DSK_KV_BF16) {
+    const uint32_t v = reinterpret_cast<const uint16_t*>(a.v_pool)[(int64_t)tok * HD + d];
+    apart = (v & 0x7f80u) == 0x7f80u;
+    return v;
+  } else {
+    const uint32_t z = a.v_sb[(int64_t)tok * (HD / 64) + d / 64];
+    uint32_t c;
+    if constexpr (KVT == DSK_KV_U8) {
+      c = reinterpret_cast<const uint8_t*>(a.v_pool)[(int64_t)tok * HD + d];
+    } else {
+      const uint32_t blk = tok & ~31u;  // pages are whole blocks
+      c = reinterpret_cast<const uint8_t*>(a.v_pool)[(int64_t)blk * (HD / 2) + kv4_v_byte(HD, (int)(tok - blk), d)];
+      c = d & 16 ? c >> 4 : c & 15;
+    }
+    const uint32_t v = f32_to_bf16(fmaf(bits_f32(z << 16), (float)c, bits_f32(z & 0xffff0000u)));
+    apart = KVT == DSK_KV_U4 ? wide2(z) : (v & 0x7f80u) == 0x7f80u;
+    return v;
+  }
+}
+// Infinities and NaN in V where not every query sees every key: a probability of 0 would not keep them out of a
+// product (4-bit codes: all of a group whose scale or offset could reach them). Such operands are staged without them, and each is added here to the queries that see its key
+// (tok: the block's first pool token). Rare, and apart from the products, which stay one run of instructions.
+template <int HD, int KVT, int TPW, int TERMS>
+__device__ __forceinline__ void add_nonfinite(const SinkArgs& a, Tile<HD, TERMS> (&tile)[TPW], const Sight (&see)[TPW],
+                                              const u32x4 (&t)[TPW][TERMS], int base, uint32_t tok, int lane) {
+#pragma unroll 1
+  for (int k = 0; k < 32; ++k) {
+    const int e = (k / 16) * 4 + k % 4, from = (lane & 15) + 16 * ((k % 16) / 4);
+    float p[TPW];
+    bool vis[TPW];
+#pragma unroll
+    for (int u = 0; u < TPW; ++u) {
+      p[u] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < TERMS; ++i) {
+        const uint32_t w = e < 4 ? (e < 2 ? t[u][i][0] : t[u][i][1]) : (e < 6 ? t[u][i][2] : t[u][i][3]);
+        p[u] += bits_f32((w << (e & 1 ? 0 : 16)) & 0xffff0000u);
+      }
+      p[u] = __shfl(p[u], from, 64);
+      vis[u] = see[u].sees(base + k);
+    }
+#pragma unroll
+    for (int d = 0; d < HD / 16; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        bool apart;
+        const uint32_t v = v_value<HD, KVT>(a, tok + k, 16 * d + 4 * (lane >> 4) + r, apart);
+#pragma unroll
+        for (int u = 0; u < TPW; ++u)
+          tile[u].o[d][r] = (int)apart & (int)vis[u] ? fmaf(p[u], bits_f32(v << 16), tile[u].o[d][r]) : tile[u].o[d][r];
+      }
+  }
 }
 
 // masks of a 32-key block's (or two blocks') scores: lane holds keys base + 16 t + 4 g + r
@@ -363,7 +397,7 @@ struct V4Raw {
 #pragma unroll
     for (int e = 0; e < 8; ++e) sb[e] = src[(16 * (e / 4) + e % 4) * (HD / 64)];
   }
-  // d tiles 4 c + 2 p + h; dead keys' words cleared before
+  // d tiles 4 c + 2 p + h
   __device__ __forceinline__ void operands(u32x4 (&v)[4]) const {
     Kv4Scale z[8];
 #pragma unroll
@@ -377,11 +411,17 @@ struct V4Raw {
       v[2 * p + 1] = u32x4{hi[0][0], hi[0][1], hi[1][0], hi[1][1]};
     }
   }
-  __device__ __forceinline__ void drop_dead(const SinkArgs& a, const KeyPlan& p, int base, int lane) {
+  // the words of keys that no query sees cleared, and the wide ones; whether there were such
+  __device__ __forceinline__ bool clean(const SinkArgs& a, const KeyPlan& p, int base, int lane) {
     asm volatile("" : "+s"(base));  // keeps the tests inside the caller's branch
+    bool bad = false;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < 8; ++e) {
       sb[e] = key_dead(a, p, base + 16 * (e / 4) + 4 * (lane >> 4) + e % 4) ? 0u : sb[e];
+      bad |= wide2(sb[e]);
+      sb[e] = wide2(sb[e]) ? 0u : sb[e];
+    }
+    return bad;
   }
 };
 
@@ -404,16 +444,22 @@ struct V4Block {
 #pragma unroll
     for (int x = 0; x < HD / 64; ++x) asm volatile("" : "+v"(q[x]), "+v"(sb[0][x]), "+v"(sb[1][x]));
   }
-  __device__ __forceinline__ void drop_dead(const SinkArgs& a, const KeyPlan& p, int base, int lane) {
-    asm volatile("" : "+s"(base));  // keeps the tests inside the caller's branch
+  __device__ __forceinline__ bool clean(const SinkArgs& a, const KeyPlan& p, int base, int lane) {  // as V4Raw::clean
+    asm volatile("" : "+s"(base));
+    bool bad = false;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const uint32_t keep = key_dead(a, p, base + 16 * u + 4 * (lane >> 4) + r) ? 0u : ~0u;
 #pragma unroll
-        for (int c = 0; c < HD / 64; ++c) sb[u][(r * (HD / 64) + c) / 4][(r * (HD / 64) + c) % 4] &= keep;
+        for (int c = 0; c < HD / 64; ++c) {
+          uint32_t w = sb[u][(r * (HD / 64) + c) / 4][(r * (HD / 64) + c) % 4] & keep;
+          bad |= wide2(w);
+          sb[u][(r * (HD / 64) + c) / 4][(r * (HD / 64) + c) % 4] = wide2(w) ? 0u : w;
+        }
       }
+    return bad;
   }
   // d tiles 4 c + 2 p + h
   __device__ __forceinline__ void operands(int c, u32x4 (&v)[4]) const {
@@ -465,12 +511,11 @@ struct VRowsRaw {
     else asm volatile("" : "+v"(h[0]), "+v"(h[1]), "+v"(h[2]), "+v"(h[3]));
     if constexpr (kBytes) asm volatile("" : "+v"(sb[0]), "+v"(sb[1]), "+v"(sb[2]), "+v"(sb[3]));
   }
-  // base: the block's first key; dst: the block's operands in LDS
-  __device__ __forceinline__ void store(const SinkArgs& a, const KeyPlan& p, int base, int quad, int ch, bool check,
+  // base: the block's first key; dst: the block's operands in LDS. check: without the keys that no query sees
+  // and what is not finite; whether there was such
+  __device__ __forceinline__ bool store(const SinkArgs& a, const KeyPlan& p, int base, int quad, int ch, bool check,
                                         uint8_t* dst) const {
-    uint32_t keep[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) keep[r] = check && key_dead(a, p, base + 4 * quad + r) ? 0u : ~0u;
+    bool bad = false;
 #pragma unroll
     for (int half = 0; half < C / 8; ++half) {
       const int ch8 = C / 8 * ch + half;
@@ -480,7 +525,17 @@ struct VRowsRaw {
         if constexpr (!kBytes) w[r] = q[r];
         else if constexpr (C == 16) w[r] = kv8_row8(q[r][2 * half], q[r][2 * half + 1], sb[r]);
         else w[r] = kv8_row8(h[r][0], h[r][1], sb[r]);
-        w[r] &= u32x4{keep[r], keep[r], keep[r], keep[r]};
+      }
+      if (check) {
+        int b0 = base;
+        asm volatile("" : "+s"(b0));  // keeps the tests inside this branch
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t keep = key_dead(a, p, b0 + 4 * quad + r) ? 0u : ~0u;
+          w[r] &= u32x4{keep, keep, keep, keep};
+          bad |= nonfinite2(w[r][0]) || nonfinite2(w[r][1]) || nonfinite2(w[r][2]) || nonfinite2(w[r][3]);
+          w[r] = finite_only(w[r]);
+        }
       }
       uint8_t* o = dst + (ch8 / 2) * kVTile + (quad % 4) * kVGroup + (ch8 % 2) * 128 + (quad / 4) * 8;
 #pragma unroll
@@ -490,6 +545,7 @@ struct VRowsRaw {
                                                       __builtin_amdgcn_perm(w[3][e / 2], w[2][e / 2], sel)};
       }
     }
+    return bad;
   }
 };
 
@@ -519,7 +575,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ?
   const int ri = a.by_G.quot(rc);
   const int pos = p.off + ri, pos_lo = p.off + a.by_G.quot(r0), pos_hi = p.off + a.by_G.quot(min(r0 + 16, a.R) - 1);
   const float c2 = (a.softcap > 0.0f ? 1.0f : a.scale) * kLog2e;
-  const Sight see = sight(a, p, pos);
+  const Sight see[1] = {sight(a, p, pos)};
 
   const int nblk = t.v1 > t.v0 + wv ? (t.v1 - t.v0 - wv + 3) / 4 : 0;  // this wave's blocks v0 + wv + 4 i
   uint32_t toks = 0;  // lane l: pool token of block (i & ~63) + l
@@ -552,7 +608,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ?
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(src + KRaw<HD, KVT>::dim(s, g));
   }
-  Tile<HD, 3> tile;
+  Tile<HD, 3> tiles[1];
+  Tile<HD, 3>& tile = tiles[0];
   tile.clear();
   uint8_t* vlds = lds + wv * DT * kVTile;
   if (nblk > 0) {  // the loop within: around it, the count of loads in flight would have to hold for no loads too
@@ -573,6 +630,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ?
       // the next block (this one again at the end: a load that may not happen would have to be waited for as
       // if it did not)
       const int nx = min(i + 1, nblk - 1);
+      const uint32_t tok_now = token(i);
       if (nx > i && (nx & 63) == 0) find_tokens(nx);
       const uint32_t tok_nx = token(nx);
       kraw.load(a, tok_nx, lane);
@@ -582,21 +640,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ?
 #pragma unroll
           for (int e = 0; e < 4; ++e) st[x][e] = tanhf(st[x][e] * a.scale / a.softcap) * a.softcap;
       }
-      if (!open) mask_scores(see, st, 0, base, g);
-      tile.soften(st, c2);
-      u32x4 pt[3];
-      Tile<HD, 3>::terms(st[0], st[1], pt);
+      if (!open) mask_scores(see[0], st, 0, base, g);
+      const float mx = tile.largest(st, c2);
+      if (__any(tile.passes(mx))) tile.raise(mx);
+      tile.soften(st[0], st[1], c2);
+      u32x4 pt[1][3];
+      Tile<HD, 3>::terms(st[0], st[1], pt[0]);
+      bool bad = false;
       if constexpr (kRows) {
 #pragma unroll
         for (int u = 0; u < NI; ++u) {
           vr[u].pin();
-          vr[u].store(a, p, base, quad_of(lane + 64 * u), chunk_of(lane + 64 * u), !open, vlds);
+          bad |= vr[u].store(a, p, base, quad_of(lane + 64 * u), chunk_of(lane + 64 * u), !open, vlds);
         }
         asm volatile("" ::: "memory");  // a wave's LDS accesses run in order; keep the compiler's order too
       } else {
         v4.pin();
-        if (!open) v4.drop_dead(a, p, base, lane);
+        if (!open) bad = v4.clean(a, p, base, lane);
       }
+      if (!open && __any(bad)) add_nonfinite<HD, KVT>(a, tiles, see, pt, base, tok_now, lane);
       static_for<DT / 4>([&](auto q) {
         constexpr int Q = decltype(q)::value, D = 4 * Q;
         u32x4 y[4];
@@ -606,21 +668,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ?
         } else {
           v4.operands(Q, y);
         }
-        if (!open && any_nonfinite(y)) {
-          tile.template add_nonfinite<D>(see, base, lane, pt, [&](int d, int k, int gg, int rr) -> uint32_t {
-            const int e = (k / 16) * 4 + k % 4, at = 4 * gg + rr + 16 * ((k % 16) / 4);  // the lane that holds it
-            if constexpr (kRows) {
-              return *reinterpret_cast<const uint16_t*>(vlds + (D + d) * kVTile + (at >> 4) * kVGroup + (at & 15) * 16 + 2 * e);
-            } else {
-              const u32x4& z = y[d];
-              const uint32_t w = __shfl(e < 4 ? (e < 2 ? z[0] : z[1]) : (e < 6 ? z[2] : z[3]), at, 64);
-              return e & 1 ? w >> 16 : w & 0xffffu;
-            }
-          });
-#pragma unroll
-          for (int d = 0; d < 4; ++d) y[d] = finite_only(y[d]);
-        }
-        tile.template add4<D>(y, pt);
+        tile.template add4<D>(y, pt[0]);
       });
       if constexpr (kRows) asm volatile("" ::: "memory");
       load_v(tok_nx);
@@ -680,6 +728,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   constexpr int kKBytes = NKT * KS * 1024, kVBytes = NB * DT * kVTile;
   __shared__ __attribute__((aligned(16))) uint8_t kbuf[2][kKBytes];
   __shared__ __attribute__((aligned(16))) uint8_t vbuf[2][kVBytes];
+  __shared__ int vbad[2][4];  // whether the V unit of a wave held something that is not finite
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const int w4 = wv & 3;
   const bool do_k = NW == 4 || wv < 4, do_v = NW == 4 || wv >= 4;
@@ -691,6 +740,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const int r0 = group * a.grows + wv * TPW * 16;
   const bool wave_live = r0 < a.R;
   const int pos_lo = p.off + a.by_G.quot(min(r0, a.R - 1)), pos_hi = p.off + a.by_G.quot(min(r0 + TPW * 16, a.R) - 1);
+  // positions of the workgroup's rows: what all of them see is staged as it is
+  const int g_lo = p.off + a.by_G.quot(group * a.grows), g_hi = p.off + a.by_G.quot(min(a.R, (group + 1) * a.grows) - 1);
   const float c2 = (a.softcap > 0.0f ? 1.0f : a.scale) * kLog2e;
   const int nch = t.v1 > t.v0 ? (t.v1 - t.v0 + NB - 1) / NB : 0;
 
@@ -712,13 +763,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   V4Raw<HD> v4;
   VRowsRaw<HD, KVT> vr;
   uint32_t tok_next[NB];  // tokens of the chunk to issue next
+  auto pool_token = [&](int base) {
+    const int lp = a.by_page.quot(base), pg = a.block_table[(int64_t)t.b * a.max_pages + lp];
+    return ((uint32_t)pg * a.nkv + kvh) * a.page + (base - lp * a.page);
+  };
   auto find = [&](int c) {
 #pragma unroll
-    for (int u = 0; u < NB; ++u) {
-      const int base = p.base(min(t.v0 + c * NB + u, t.v1 - 1));
-      const int lp = a.by_page.quot(base), pg = a.block_table[(int64_t)t.b * a.max_pages + lp];
-      tok_next[u] = ((uint32_t)pg * a.nkv + kvh) * a.page + (base - lp * a.page);
-    }
+    for (int u = 0; u < NB; ++u) tok_next[u] = pool_token(p.base(min(t.v0 + c * NB + u, t.v1 - 1)));
   };
   // U4 K unit w4: tile w4 (head_dim 128: of 64 keys), or tile w4 / 2, half w4 % 2 (256); V unit: chunk w4 % (HD / 64) of block w4 / (HD / 64)
   constexpr int kHalves = HD / 128;
@@ -769,17 +820,20 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     if (do_v) {
       const int blk = kRows ? vblk : vb, v = t.v0 + c * NB + blk;
       const int base = v < t.v1 ? p.base(v) : 0x40000000;  // past the split: every key dead
-      const bool check = base + 31 >= p.j_end || base < p.j_beg;
+      const bool check = !block_open(a, p, base, g_lo, g_hi);
+      bool bad = false;
       if constexpr (kRows) {
-        vr.store(a, p, base, vq, vch, check, &vbuf[buf][blk * DT * kVTile]);
+        bad = vr.store(a, p, base, vq, vch, check, &vbuf[buf][blk * DT * kVTile]);
       } else {
-        if (check) v4.drop_dead(a, p, base, lane);
+        if (check) bad = v4.clean(a, p, base, lane);
         u32x4 x[4];
         v4.operands(x);
 #pragma unroll
         for (int d = 0; d < 4; ++d)
           *reinterpret_cast<u32x4*>(&vbuf[buf][(blk * DT + 4 * vc + d) * kVTile + g * kVGroup + n * 16]) = x[d];
       }
+      const int any_bad = __any(bad);
+      if (lane == 0) vbad[buf][w4] = any_bad;
     }
   };
 
@@ -811,7 +865,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
         for (int u = 0; u < TPW; ++u) st[u][x] = mfma16(kf, qf[u][s], st[u][x]);
       }
-    u32x4 pt[TPW][NB][TERMS];
+    float mx[TPW];
+    bool up = false;
 #pragma unroll
     for (int u = 0; u < TPW; ++u) {
       if (a.softcap > 0.0f) {
@@ -824,32 +879,47 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
         for (int x = 0; x < NB; ++x) mask_scores(see[u], st[u], 2 * x, base[x], g);
       }
-      tile[u].soften(st[u], c2);
-#pragma unroll
-      for (int x = 0; x < NB; ++x) Tile<HD, TERMS>::terms(st[u][2 * x], st[u][2 * x + 1], pt[u][x]);
+      mx[u] = tile[u].largest(st[u], c2);
+      up |= tile[u].passes(mx[u]);
     }
+    if (__any(up)) {
 #pragma unroll
-    for (int x = 0; x < NB; ++x) {
+      for (int u = 0; u < TPW; ++u) tile[u].raise(mx[u]);
+    }
+    // a block's exponentials are among the products of the one before
+    u32x4 pt[NB][TPW][TERMS];
+    auto weigh = [&](auto xc) {
+      constexpr int x = decltype(xc)::value;
+#pragma unroll
+      for (int u = 0; u < TPW; ++u) {
+        tile[u].soften(st[u][2 * x], st[u][2 * x + 1], c2);
+        Tile<HD, TERMS>::terms(st[u][2 * x], st[u][2 * x + 1], pt[x][u]);
+      }
+    };
+    auto guard = [&](auto xc) {
+      constexpr int x = decltype(xc)::value;
+      if (open) return;
+      bool bad = false;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) bad |= (kRows ? w * 64 / (16 * DT) : w / (HD / 64)) == x && vbad[buf][w];
+      if (bad) add_nonfinite<HD, KVT>(a, tile, see, pt[x], base[x], pool_token(base[x]), lane);
+    };
+    weigh(std::integral_constant<int, 0>{});
+    guard(std::integral_constant<int, 0>{});
+    static_for<NB>([&](auto xc) {
+      constexpr int x = decltype(xc)::value;
+      if constexpr (x + 1 < NB) weigh(std::integral_constant<int, x + 1>{});
       const uint8_t* vb8 = &vbuf[buf][x * DT * kVTile];
       static_for<DT / 4>([&](auto q) {
         constexpr int D = 4 * decltype(q)::value;
         u32x4 w[4];
 #pragma unroll
         for (int d = 0; d < 4; ++d) w[d] = v_operand(vb8, D + d, lane);
-        if (!open && any_nonfinite(w)) {
 #pragma unroll
-          for (int u = 0; u < TPW; ++u)
-            tile[u].template add_nonfinite<D>(see[u], base[x], lane, pt[u][x], [&](int d, int k, int gg, int rr) -> uint32_t {
-              return *reinterpret_cast<const uint16_t*>(vb8 + (D + d) * kVTile + ((k % 16) / 4) * kVGroup + (4 * gg + rr) * 16 +
-                                                        2 * ((k / 16) * 4 + k % 4));
-            });
-#pragma unroll
-          for (int d = 0; d < 4; ++d) w[d] = finite_only(w[d]);
-        }
-#pragma unroll
-        for (int u = 0; u < TPW; ++u) tile[u].template add4<D>(w, pt[u][x]);
+        for (int u = 0; u < TPW; ++u) tile[u].template add4<D>(w, pt[x][u]);
       });
-    }
+      if constexpr (x + 1 < NB) guard(std::integral_constant<int, x + 1>{});
+    });
   };
 
   if (nch > 0) {
@@ -863,13 +933,17 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     int c = 0;
 #pragma unroll 1
     do {
-      compute(c & 1, c);
+      // half of the waves stage first, so that a SIMD's two waves are not all in products or all out of them
+      // (a prompt of 4096 tokens, 32 heads of 128 dims: 289 us with all computing first, 285 so; 2048 tokens
+      // under a window of 1024, 12 heads of 256 dims: 107 and 102)
+      const bool late = wv >= NW / 2;
+      if (!late) compute(c & 1, c);
       if (c + 1 < nch) {
-        // the other buffer was last read for chunk c - 1, before the last barrier
         stage((c + 1) & 1, c + 1);
         if (c + 2 < nch) issue();
         if (c + 3 < nch) find(c + 3);
       }
+      if (late) compute(c & 1, c);
       __syncthreads();
     } while (++c < nch);
   }

@@ -197,6 +197,23 @@ def test_values_only_some_rows_see(dev, bits, hd, nq, nkv, W, n, window, sinks):
     check(run(dev, c, q, [n], W, nq, nkv, True, window, sinks, rows=W > 64), want, tol)
 
 
+@pytest.mark.parametrize("hd,nq,nkv,W", [(128, 4, 2, 5), (256, 4, 2, 9), (128, 8, 2, 70)])
+def test_values_past_the_range_of_four_bits(dev, hd, nq, nkv, W):
+    """A scale and offset that are finite, whose values are not (15 * 2^125 + 2^125), in the newest token: the
+    rows before do not see it, the last one does (all its values are 2^125 or more)."""
+    print(f"wide hd={hd} W={W}", flush=True)
+    n = 70
+    c = Cache(4, 1, nkv, hd, -(-(n + W) // 64), 64, seed=3)
+    q = queries(1, W, nq, hd, 2)
+    pg, sl = int(c.table[0][(n + W - 1) // 64]), (n + W - 1) % 64
+    c.sbs[1][pg, :, sl] = 0x7E007E00
+    c.vals[1][pg, :, sl] = 0.0
+    want, tol = reference(c, q, [n], W, nq, nkv, True, 0, 0, hd ** -0.5)
+    got = run(dev, c, q, [n], W, nq, nkv, rows=W > 64)
+    check(got[:, :-1], want[:, :-1], tol[:, :-1])
+    assert (~got[:, -1].isfinite() | (got[:, -1].abs() > 2.0 ** 90)).all()
+
+
 @pytest.mark.parametrize("W,nq,nkv,hd", [(1, 4, 2, 128), (9, 16, 8, 256), (70, 8, 2, 128)])
 def test_softcap_scale_and_sharp_scores(dev, W, nq, nkv, hd):
     """Soft-capped scores, another scale, and scores so large that the maximum moves block after block."""
