@@ -87,13 +87,36 @@ struct SplitTask {
   int b, slot, v0, v1, live;
   KeyPlan p;
 };
-// The rows' lengths, one per lane (one load for all: read one after the other they cost a round trip each).
-__device__ __forceinline__ int row_lengths(const SinkArgs& a) { return a.seq_lens[min((int)(threadIdx.x & 63), a.B - 1)]; }
-__device__ __forceinline__ int balanced_blocks(const SinkArgs& a, int lens) {
-  int total = 0;
-  for (int b = 0; b < a.B; ++b) total += key_plan(a, __builtin_amdgcn_readlane(lens, b), 0, a.W - 1).T;
-  // sum of ceil(T / bps) <= (slots - B) + B
-  return max(kSplitUnit, ((total + a.slots - a.B - 1) / (a.slots - a.B) + kSplitUnit - 1) & -kSplitUnit);
+// Rows by their lengths, one row per lane (one load for all: read one after the other they cost a round trip
+// each): the fewest blocks per split, in units, with which the rows' splits fit the slots, and the lane's row's
+// number of splits. sum ceil(T / bps) <= sum T / bps + B gives one that fits; a few halvings from the ideal
+// sum T / slots find a better one (32 rows of 4096 keys, 32 heads: 75 us with the first, 53 so).
+struct Placement {
+  int lens, live, bps;
+};
+__device__ __forceinline__ Placement placement(const SinkArgs& a) {
+  const int lane = threadIdx.x & 63;
+  Placement p;
+  p.lens = a.seq_lens[min(lane, a.B - 1)];
+  const int T = key_plan(a, p.lens, 0, a.W - 1).T;
+  auto sum = [&](int x) {
+    int s = 0;
+    for (int b = 0; b < a.B; ++b) s += __builtin_amdgcn_readlane(x, b);
+    return s;
+  };
+  auto units = [](int x) { return max(kSplitUnit, (x + kSplitUnit - 1) & -kSplitUnit); };
+  auto splits = [&](int bps) { return max(1, (int)((uint32_t)(T + bps - 1) / (uint32_t)bps)); };
+  const int total = sum(T);
+  int lo = units((int)((uint32_t)(total + a.slots - 1) / (uint32_t)a.slots));
+  p.bps = units((int)((uint32_t)(total + a.slots - a.B - 1) / (uint32_t)(a.slots - a.B)));
+#pragma unroll 1
+  for (int i = 0; i < 4 && lo < p.bps; ++i) {
+    const int x = i == 0 ? lo : units((lo + p.bps) / 2 - kSplitUnit + 1);
+    if (sum(splits(x)) <= a.slots) p.bps = x;
+    else lo = x + kSplitUnit;
+  }
+  p.live = splits(p.bps);
+  return p;
 }
 __device__ __forceinline__ int even_blocks(const SinkArgs& a, int T) {
   return max(kSplitUnit, (a.by_nsplit.quot(T + a.nsplit - 1) + kSplitUnit - 1) & -kSplitUnit);
@@ -103,17 +126,16 @@ __device__ __forceinline__ SplitTask split_task(const SinkArgs& a, int slot, int
   t.slot = slot;
   t.live = 0;
   if (a.balanced) {
-    const int lens = row_lengths(a), bps = balanced_blocks(a, lens);
+    const Placement pl = placement(a);
     int first = 0;
     for (int b = 0; b < a.B; ++b) {
-      const KeyPlan p = key_plan(a, __builtin_amdgcn_readlane(lens, b), 0, a.W - 1);
-      const int live = max(1, (p.T + bps - 1) / bps);
+      const int live = __builtin_amdgcn_readlane(pl.live, b);
       if (slot < first + live) {
         t.b = b;
-        t.p = p;
+        t.p = key_plan(a, __builtin_amdgcn_readlane(pl.lens, b), 0, a.W - 1);
         t.live = live;
-        t.v0 = (slot - first) * bps;
-        t.v1 = min(p.T, t.v0 + bps);
+        t.v0 = (slot - first) * pl.bps;
+        t.v1 = min(t.p.T, t.v0 + pl.bps);
         break;
       }
       first += live;
@@ -559,8 +581,12 @@ __device__ __forceinline__ u32x4 v_operand(const uint8_t* blk, int d, int lane) 
 // own operands (4-bit V lies in operand order; row-major V is transposed through the wave's LDS).
 // Page ids of 64 blocks are loaded at once, one per lane.
 
+// Waves per SIMD: at head_dim 256 only 4-bit codes fit 256 registers (8 rows of 8192: 66 us with one, 55 with
+// two); the others would spill.
+template <int HD, int KVT> constexpr int kTileWaves = HD == 128 || KVT == DSK_KV_U4 ? 2 : 1;
+
 template <int HD, int KVT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 2 : 1, 2))) void attention_tile_kernel(SinkArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<HD, KVT>, 2))) void attention_tile_kernel(SinkArgs a) {
   constexpr int KS = HD / 32, DT = HD / 16;
   constexpr int VC = KVT == DSK_KV_U8 ? 16 : 8, NI = HD / VC / 8;  // V items (4 keys x VC dims) per lane
   constexpr bool kRows = KVT != DSK_KV_U4;
@@ -983,10 +1009,10 @@ __global__ __launch_bounds__(256) void attention_join_kernel(SinkArgs a) {
   const int ch = threadIdx.x % C, sl = threadIdx.x / C;
   int first, live;
   if (a.balanced) {
-    const int lens = row_lengths(a), bps = balanced_blocks(a, lens);
+    const Placement pl = placement(a);
     first = 0;
-    for (int x = 0; x < b; ++x) first += max(1, (key_plan(a, __builtin_amdgcn_readlane(lens, x), 0, a.W - 1).T + bps - 1) / bps);
-    live = max(1, (key_plan(a, __builtin_amdgcn_readlane(lens, b), 0, a.W - 1).T + bps - 1) / bps);
+    for (int x = 0; x < b; ++x) first += __builtin_amdgcn_readlane(pl.live, x);
+    live = __builtin_amdgcn_readlane(pl.live, b);
   } else {
     const int group = r / a.grows;
     const int T = key_plan(a, a.seq_lens[b], a.by_G.quot(group * a.grows), a.by_G.quot(min(a.R, (group + 1) * a.grows) - 1)).T;
@@ -1052,7 +1078,8 @@ struct SinkPlan {
   int waves, tpw;  // block kernel
   int groups, grows, nsplit, balanced, slots;
 };
-static SinkPlan sink_plan(int B, int W, int nq, int nkv, int hd, int causal, int window, int sinks, int max_ctx) {
+static SinkPlan sink_plan(int B, int W, int nq, int nkv, int hd, int causal, int window, int sinks, int max_ctx,
+                          int kv_dtype) {
   SinkPlan s = {};
   const int64_t R = (int64_t)W * (nq / nkv);
   s.tile = R <= 16;
@@ -1067,18 +1094,20 @@ static SinkPlan sink_plan(int B, int W, int nq, int nkv, int hd, int causal, int
   int64_t span = max_ctx;
   if (causal && window > 0) span = std::min<int64_t>(span, (int64_t)window + W + sinks + 96);
   const int64_t most = std::max<int64_t>(1, ceil_div(ceil_div(span, 32) + 1, kSplitUnit));
-  // workgroups that run at once: two per CU, one of the tile kernel at head_dim 256 (its registers)
-  const int64_t tasks = (int64_t)B * nkv * s.groups, want = s.tile && hd == 256 ? 256 : 512;
+  // workgroups that run at once: two per CU, one of the tile kernel with one wave per SIMD
+  const bool one = s.tile && hd == 256 && kv_dtype != DSK_KV_U4;
+  const int64_t tasks = (int64_t)B * nkv * s.groups, want = one ? 256 : 512;
   s.nsplit = (int)std::min<int64_t>(most, std::max<int64_t>(1, want / tasks));
-  s.balanced = s.groups == 1 && B <= kBalancedRows && B > 1 && s.nsplit > 1;
   s.slots = B * s.nsplit;
+  if (s.groups == 1 && B <= kBalancedRows && B > 1) s.slots = (int)std::min<int64_t>(B * most, std::max<int64_t>(B, want / nkv));
+  s.balanced = s.slots > B && s.groups == 1 && B <= kBalancedRows && B > 1;
   return s;
 }
 static size_t sink_part_o_bytes(const SinkPlan& s, int64_t R, int nkv, int hd) {
   return ((size_t)s.slots * nkv * R * hd * sizeof(float) + 255) & ~(size_t)255;
 }
-static size_t sink_ws(const SinkPlan& s, int64_t R, int nkv, int hd) {
-  return s.nsplit > 1 ? sink_part_o_bytes(s, R, nkv, hd) + (size_t)s.slots * nkv * R * 2 * sizeof(float) : 0;
+static size_t sink_ws(const SinkPlan& s, int B, int64_t R, int nkv, int hd) {
+  return s.slots > B ? sink_part_o_bytes(s, R, nkv, hd) + (size_t)s.slots * nkv * R * 2 * sizeof(float) : 0;
 }
 
 template <int HD, int KVT>
@@ -1096,7 +1125,7 @@ static void launch_sinks(const SinkArgs& a, const SinkPlan& s, int terms, hipStr
   } else {
     hipLaunchKernelGGL((attention_block_kernel<HD, KVT, 4, 1, 3>), grid, dim3(256), 0, st, a);
   }
-  if (s.nsplit > 1)
+  if (s.slots > a.B)
     hipLaunchKernelGGL((attention_join_kernel<HD>), dim3((unsigned)a.R, (unsigned)(a.B * a.nkv)), dim3(256), 0, st, a);
 }
 
@@ -1108,7 +1137,10 @@ extern "C" size_t dsk_attention_sinks_ws_bytes(int B, int W, int nq, int nkv, in
                                                int max_ctx) {
   if (B <= 0 || W <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || (hd != 128 && hd != 256) || max_ctx <= 0 || window < 0 || sinks < 0)
     return 0;
-  return sink_ws(sink_plan(B, W, nq, nkv, hd, causal, window, sinks, max_ctx), (int64_t)W * (nq / nkv), nkv, hd);
+  size_t most = 0;  // of the cache types
+  for (int kv : {DSK_KV_BF16, DSK_KV_U8, DSK_KV_U4})
+    most = std::max(most, sink_ws(sink_plan(B, W, nq, nkv, hd, causal, window, sinks, max_ctx, kv), B, (int64_t)W * (nq / nkv), nkv, hd));
+  return most;
 }
 
 extern "C" int dsk_attention_sinks(const uint16_t* q, int B, int W, int nq, int nkv, int hd, float scale, int causal,
@@ -1135,10 +1167,10 @@ extern "C" int dsk_attention_sinks(const uint16_t* q, int B, int W, int nq, int 
               "%s: q, pools and out must be 16-byte aligned", who);
   DSK_REQUIRE(!out_packed || (B * W <= 64 && (nq * hd) % 64 == 0), "%s: packed output needs B*W <= 64", who);
   const int64_t R = (int64_t)W * (nq / nkv);
-  const SinkPlan s = sink_plan(B, W, nq, nkv, hd, causal, window, sinks, max_ctx);
+  const SinkPlan s = sink_plan(B, W, nq, nkv, hd, causal, window, sinks, max_ctx, kv_dtype);
   DSK_REQUIRE(R <= 0x7fffffff && s.groups <= 65535 && (int64_t)s.slots * nkv <= 0x7fffffff && (int64_t)B * nkv <= 65535,
               "%s: %lld query rows per kv head", who, (long long)R);
-  const size_t need = sink_ws(s, R, nkv, hd);
+  const size_t need = sink_ws(s, B, R, nkv, hd);
   if (need && (!workspace || ws_bytes < need)) {
     set_error("%s: workspace %zu < %zu", who, ws_bytes, need);
     return DSK_ENOWS;

@@ -261,6 +261,19 @@ def test_many_rows_batch(dev):
     check(run(dev, c, q, lens, 1, 2, 1), want, tol)
 
 
+@pytest.mark.parametrize("B,W,hd,bits,window,sinks", [(40, 1, 128, 4, 0, 0), (33, 2, 128, 8, 600, 4), (12, 1, 256, 4, 0, 0),
+                                                   (12, 1, 256, 0, 900, 8), (64, 1, 128, 4, 0, 0), (65, 1, 128, 4, 0, 0)])
+def test_one_long_row_among_short_ones(dev, B, W, hd, bits, window, sinks):
+    """Splits are placed by the rows' lengths: one row gets most of them, empty rows one each."""
+    print(f"placement B={B} W={W} hd={hd} bits={bits}", flush=True)
+    lens = [(7 * b) % 40 for b in range(B)]
+    lens[B // 2] = 1500
+    c = Cache(bits, B, 8, hd, 24, 64, seed=B)
+    q = queries(B, W, 8, hd, 5)
+    want, tol = reference(c, q, lens, W, 8, 8, True, window, sinks, hd ** -0.5)
+    check(run(dev, c, q, lens, W, 8, 8, True, window, sinks), want, tol)
+
+
 @pytest.mark.parametrize("bits,window,sinks,W", [(4, 0, 0, 1), (4, 64, 4, 9), (8, 64, 4, 1)])
 def test_graph_replay_follows_lengths(dev, bits, window, sinks, W):
     """A captured append + attention replayed while the device lengths advance, against the eager calls; a
