@@ -51,6 +51,7 @@ struct SinkArgs {
   int nsplit, balanced;
   float* part_o;   // [slot][kv head][R][HD] unnormalised outputs
   float* part_ml;  // [slot][kv head][R][2] running maximum (of scores times c2) and sum
+  int2* part_at;   // [row b] first slot and number of splits (balanced)
   FastDiv by_page, by_G, by_nkv, by_nsplit;
 };
 
@@ -136,6 +137,8 @@ __device__ __forceinline__ SplitTask split_task(const SinkArgs& a, int slot, int
         t.live = live;
         t.v0 = (slot - first) * pl.bps;
         t.v1 = min(t.p.T, t.v0 + pl.bps);
+        // for the join: its many workgroups would take longer to place the rows again than to read this
+        if (slot == first && group == 0 && slot * a.nkv == (int)blockIdx.x && threadIdx.x == 0) a.part_at[b] = int2{first, live};
         break;
       }
       first += live;
@@ -1009,10 +1012,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(SinkArgs a) {
   const int ch = threadIdx.x % C, sl = threadIdx.x / C;
   int first, live;
   if (a.balanced) {
-    const Placement pl = placement(a);
-    first = 0;
-    for (int x = 0; x < b; ++x) first += __builtin_amdgcn_readlane(pl.live, x);
-    live = __builtin_amdgcn_readlane(pl.live, b);
+    const int2 at = a.part_at[b];
+    first = at.x;
+    live = at.y;
   } else {
     const int group = r / a.grows;
     const int T = key_plan(a, a.seq_lens[b], a.by_G.quot(group * a.grows), a.by_G.quot(min(a.R, (group + 1) * a.grows) - 1)).T;
@@ -1082,32 +1084,44 @@ static SinkPlan sink_plan(int B, int W, int nq, int nkv, int hd, int causal, int
                           int kv_dtype) {
   SinkPlan s = {};
   const int64_t R = (int64_t)W * (nq / nkv);
-  s.tile = R <= 16;
+  // Few rows: a workgroup per 16 rows, each reading the keys again, keeps more of the chip at work than one with
+  // idle waves (us, tiles / blocks, contexts of 4096, 32 heads of 128: 8 x 8 new tokens over 4-bit codes 31 / 40,
+  // 32 x 8 81 / 131, 32 x 9 118 / 137, 8 x 16 48 / 47; 16 x 8 over 8-bit ones in a window of 4096 59 / 76, 16 x 9
+  // 85 / 81; over bf16 91 / 74, at 256 dims in a window of 1024 28 / 34).
+  s.tile = R <= (kv_dtype == DSK_KV_U4 ? 64 : kv_dtype == DSK_KV_U8 || hd == 256 ? 32 : 16);
+  // keys a pass may look at (the sliding window's rows, and its sinks)
+  int64_t span = max_ctx;
+  if (causal && window > 0) span = std::min<int64_t>(span, (int64_t)window + W + sinks + 96);
   if (!s.tile) {
-    const bool big = hd == 128 && R > 64;
+    // 256 rows per workgroup share a key's operands, 64 balance better: 256 where they fill the chip unsplit or
+    // there are many keys (us, 256 / 64: prompts of 4000 tokens 270 / 341, of 2048 157 / 114, of 1024 82 / 42;
+    // 1024 after 16384 543 / 728; verify passes of 17 .. 63 tokens are a tenth slower in 256)
+    const bool big = hd == 128 && R >= 256 && ((int64_t)B * nkv * ceil_div(R, 256) > 256 || span >= 4096);
     s.waves = big ? 8 : 4;
     s.tpw = big ? 2 : 1;
   }
   s.grows = s.tile ? 16 : s.waves * s.tpw * 16;
   s.groups = (int)ceil_div(R, s.grows);
-  // blocks of 32 keys a pass may look at (the sliding window's rows, and its sinks)
-  int64_t span = max_ctx;
-  if (causal && window > 0) span = std::min<int64_t>(span, (int64_t)window + W + sinks + 96);
-  const int64_t most = std::max<int64_t>(1, ceil_div(ceil_div(span, 32) + 1, kSplitUnit));
-  // workgroups that run at once: two per CU, one of the tile kernel with one wave per SIMD
-  const bool one = s.tile && hd == 256 && kv_dtype != DSK_KV_U4;
+  // Splits of many rows are 512 keys or more: their parts are written and read again (200 tokens after 4096:
+  // 86 us with at least 1024, 73 so; 512 tokens alone: 39 with at least 256, 22 so).
+  const int64_t most = std::max<int64_t>(1, !s.tile && R >= 256 ? span / 512 : ceil_div(ceil_div(span, 32) + 1, kSplitUnit));
+  // workgroups that run at once: two per CU; one of 8 waves, or of the tile kernel with one wave per SIMD
+  // (2048 tokens after 8192: 620 us planned for two, 586 so)
+  const bool one = s.tile ? hd == 256 && kv_dtype != DSK_KV_U4 : s.waves == 8;
   const int64_t tasks = (int64_t)B * nkv * s.groups, want = one ? 256 : 512;
   s.nsplit = (int)std::min<int64_t>(most, std::max<int64_t>(1, want / tasks));
   s.slots = B * s.nsplit;
-  if (s.groups == 1 && B <= kBalancedRows && B > 1) s.slots = (int)std::min<int64_t>(B * most, std::max<int64_t>(B, want / nkv));
-  s.balanced = s.slots > B && s.groups == 1 && B <= kBalancedRows && B > 1;
+  if ((s.groups == 1 || s.tile) && B <= kBalancedRows && B > 1) {
+    s.slots = (int)std::min<int64_t>(B * most, std::max<int64_t>(B, want / (nkv * s.groups)));
+    s.balanced = s.slots > B;
+  }
   return s;
 }
 static size_t sink_part_o_bytes(const SinkPlan& s, int64_t R, int nkv, int hd) {
   return ((size_t)s.slots * nkv * R * hd * sizeof(float) + 255) & ~(size_t)255;
 }
 static size_t sink_ws(const SinkPlan& s, int B, int64_t R, int nkv, int hd) {
-  return s.slots > B ? sink_part_o_bytes(s, R, nkv, hd) + (size_t)s.slots * nkv * R * 2 * sizeof(float) : 0;
+  return s.slots > B ? sink_part_o_bytes(s, R, nkv, hd) + (size_t)s.slots * nkv * R * 2 * sizeof(float) + (s.balanced ? B * sizeof(int2) : 0) : 0;
 }
 
 template <int HD, int KVT>
@@ -1180,6 +1194,8 @@ extern "C" int dsk_attention_sinks(const uint16_t* q, int B, int W, int nq, int 
                 max_pages, page, k_pool, v_pool, k_sb, v_sb, out, out_packed ? 1 : 0, s.groups, s.grows, s.slots, s.nsplit,
                 s.balanced, reinterpret_cast<float*>(workspace),
                 reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + sink_part_o_bytes(s, R, nkv, hd)),
+                reinterpret_cast<int2*>(reinterpret_cast<char*>(workspace) + sink_part_o_bytes(s, R, nkv, hd) +
+                                        (size_t)s.slots * nkv * R * 2 * sizeof(float)),
                 FastDiv(page), FastDiv(nq / nkv), FastDiv(nkv), FastDiv(s.nsplit)};
 #define DSK_SINKS(HDV)                                                                                \
   if (kv_dtype == DSK_KV_BF16) launch_sinks<HDV, DSK_KV_BF16>(a, s, p_terms, as_stream(stream));      \

@@ -262,7 +262,8 @@ def test_many_rows_batch(dev):
 
 
 @pytest.mark.parametrize("B,W,hd,bits,window,sinks", [(40, 1, 128, 4, 0, 0), (33, 2, 128, 8, 600, 4), (12, 1, 256, 4, 0, 0),
-                                                   (12, 1, 256, 0, 900, 8), (64, 1, 128, 4, 0, 0), (65, 1, 128, 4, 0, 0)])
+                                                   (12, 1, 256, 0, 900, 8), (64, 1, 128, 4, 0, 0), (65, 1, 128, 4, 0, 0),
+                                                   (3, 33, 128, 4, 0, 0), (5, 20, 128, 8, 300, 40), (2, 61, 256, 4, 0, 0)])
 def test_one_long_row_among_short_ones(dev, B, W, hd, bits, window, sinks):
     """Splits are placed by the rows' lengths: one row gets most of them, empty rows one each."""
     print(f"placement B={B} W={W} hd={hd} bits={bits}", flush=True)
