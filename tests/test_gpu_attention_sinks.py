@@ -275,6 +275,21 @@ def test_one_long_row_among_short_ones(dev, B, W, hd, bits, window, sinks):
     check(run(dev, c, q, lens, W, 8, 8, True, window, sinks), want, tol)
 
 
+@pytest.mark.parametrize("bits,nq,nkv,W,lens,window,sinks,rows", [
+    (4, 8, 2, 64, [4100], 0, 0, False), (4, 8, 2, 70, [33], 0, 0, True), (4, 16, 2, 40, [4000, 7], 0, 0, False),
+    (8, 8, 2, 90, [4060], 4060, 40, True), (0, 6, 1, 101, [4000], 4050, 3, True), (0, 8, 2, 64, [0, 4096], 4096, 1, False)])
+def test_many_rows_long_context(dev, bits, nq, nkv, W, lens, window, sinks, rows):
+    """Workgroups of 256 rows: contexts that may be 4096 long."""
+    print(f"long bits={bits} W={W} lens={lens} window={window}", flush=True)
+    c = Cache(bits, len(lens), nkv, 128, 68, 64, seed=W)
+    for b, n in enumerate(lens):
+        see = visible(n, W, n + W, True, window, sinks).any(0)
+        c.poison(b, torch.cat((torch.nonzero(~see).view(-1), torch.arange(n + W, 68 * 64))))
+    q = queries(len(lens), W, nq, 128, 5)
+    want, tol = reference(c, q, lens, W, nq, nkv, True, window, sinks, 128 ** -0.5)
+    check(run(dev, c, q, lens, W, nq, nkv, True, window, sinks, rows=rows), want, tol)
+
+
 @pytest.mark.parametrize("bits,window,sinks,W", [(4, 0, 0, 1), (4, 64, 4, 9), (8, 64, 4, 1)])
 def test_graph_replay_follows_lengths(dev, bits, window, sinks, W):
     """A captured append + attention replayed while the device lengths advance, against the eager calls; a
