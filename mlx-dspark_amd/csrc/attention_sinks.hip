@@ -186,9 +186,9 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 __device__ __forceinline__ bool nonfinite2(uint32_t w) {
   return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
-// whether 4-bit values under this scale and offset may pass the largest float (the others do not, in 32 bits)
+// whether 4-bit values under this scale and offset may leave what kv4_scale takes, or the largest float
 __device__ __forceinline__ bool wide2(uint32_t sb) {
-  return (sb & 0x7f80u) >= 0x7d00u || (sb & 0x7f800000u) >= 0x7d000000u;  // 2^123 or more: 15 s + |b| < 2^127 below
+  return (sb & 0x7f80u) >= 0x7300u || (sb & 0x7f800000u) >= 0x7d000000u;  // s >= 2^103, |b| >= 2^123
 }
 __device__ __forceinline__ int64_t sink_out_index(const SinkArgs& a, int HD, int b, int r, int kvh, int d) {
   const int i = a.by_G.quot(r);
