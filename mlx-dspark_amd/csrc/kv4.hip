@@ -7,49 +7,51 @@
 namespace dsk {
 
 // ----------------------------------------------------------------------------- append
-// q, k: x * rsqrt(mean(x^2) + eps) * w, rotated by pos * inv_freq; k and v to 4-bit codes (kv4.h). A
-// row stays float32 from its projection's sum to its code or its bf16 query: a rounding in between
-// would move about one code in a hundred.
+// q, k: x * rsqrt(mean(x^2) + eps) * w, rotated by pos * inv_freq; k and v to 4-bit codes (kv4.h). A row is not
+// rounded between its projection's sum and its code or its bf16 query: to bf16, that would move about one code
+// in a hundred. Keys are formed in 64 bits, and so are the sums of slices: in 32, a few of the codes of a
+// 2048-token prompt are not the nearest (15.9 us instead of 14.5 for 40 heads of 128 with 8 of V).
+//
+// What bounds it: few rows, the chain of loads (lengths, row, angles: 6.6 us for one token in a graph, of which
+// about 4 are two launches); many, the bytes: 44 MB for that prompt, 2.8 TB/s.
 //
 // Queries and keys: one workgroup per token row and chunk of heads; the row's HD / 2 sines and cosines are found
 // once, one per thread, for all heads of the chunk; then 8 dims per lane, HD / 8 lanes per head. V, in the same
 // launch: one workgroup per 4 positions.
 
-// sin and cos of the exact product p f (a float32 angle is off by up to 2^-25 of itself: 0.004 rad at
-// position 131072). Reduction by multiples k of pi/2 = P1 + P2 + P3: p f = a + (its fma remainder); a - k P1
-// is exact below 2^20 (both are multiples of 2^-23, the difference below 2), the rest is carried as a second
-// term through the Taylor polynomials on [-pi/4, pi/4] (their next terms are below 2^-28). Off by at most
-// 4.6e-8 over 2e7 positions below 2^20, 2.5 % of the results not the nearest float32.
-__device__ __forceinline__ void rope_exact(float p, float f, float& sn, float& cs) {
-  const float a = p * f, alo = __builtin_fmaf(p, f, -a);
-  if (fabsf(a) >= 1048576.0f) {
-    sincosf(a, &sn, &cs);
-    const float s0 = sn, one = 1.0f - 0.5f * alo * alo;
-    sn = s0 * one + cs * alo;
-    cs = cs * one - s0 * alo;
-    return;
-  }
-  const float P1 = 1.57079637e+0f, P2 = -4.37113883e-8f, P3 = -1.71512451e-15f;
-  const float k = rintf(a * 0.636619772f);
-  const float r1 = __builtin_fmaf(-k, P1, a), r2 = __builtin_fmaf(-k, P2, r1);
-  const float e = __builtin_fmaf(-k, P3, __builtin_fmaf(-k, P2, r1 - r2) + alo);
-  const float r = r2 + e, rl = fabsf(r2) >= fabsf(e) ? (r2 - r) + e : (e - r) + r2;
-  const float z = r * r, hz = 0.5f * z, w = 1.0f - hz;
-  const float ps = __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, 2.75573192e-6f, -1.98412698e-4f), 8.33333333e-3f), -1.66666667e-1f);
-  const float pc = __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, -2.75573192e-7f, 2.48015873e-5f), -1.38888889e-3f), 4.16666667e-2f);
-  const float s = r + __builtin_fmaf(r * z, ps, rl * w);
-  const float c = w + (((1.0f - w) - hz) + __builtin_fmaf(z * z, pc, -r * rl));
-  const int q = (int)k;
-  const float u = q & 1 ? c : s, v = q & 1 ? s : c;
-  sn = q & 2 ? -u : u;
-  cs = (q + 1) & 2 ? -v : v;
+// sin and cos of p f, p an integer and f a float32 (a float32 angle would be off by up to 2^-25 of itself: 0.004
+// rad at position 131072). The product is exact in 64 bits for p below 2^29. Reduction by a multiple k of pi/2 =
+// P1 + P2 (P1 its nearest double, the product inside the fma): off by 2^-53 of the remainder and k 2^-107. Then
+// the Taylor polynomials on [-pi/4, pi/4], whose next terms are 2e-17 (sin, r^17 / 17!) and 5e-17 (cos).
+__device__ __forceinline__ double2 rope_angle(double p, float f) {
+  const double a = p * (double)f, k = rint(a * 0.63661977236758134308);
+  const double r = fma(-k, 6.12323399573676588613e-17, fma(-k, 1.57079632679489661923, a)), z = r * r;
+  double s = -7.6471637318198164759e-13, c = -1.1470745597729724714e-11;
+  s = fma(s, z, 1.6059043836821614599e-10);
+  s = fma(s, z, -2.5052108385441718775e-8);
+  s = fma(s, z, 2.7557319223985890653e-6);
+  s = fma(s, z, -1.9841269841269841270e-4);
+  s = fma(s, z, 8.3333333333333333333e-3);
+  s = fma(s, z, -1.6666666666666666667e-1);
+  s = fma(s * z, r, r);
+  c = fma(4.7794773323873852974e-14, z, c);
+  c = fma(c, z, 2.0876756987868098979e-9);
+  c = fma(c, z, -2.7557319223985890653e-7);
+  c = fma(c, z, 2.4801587301587301587e-5);
+  c = fma(c, z, -1.3888888888888888889e-3);
+  c = fma(c, z, 4.1666666666666666667e-2);
+  c = fma(c, z, -0.5);
+  c = fma(c, z, 1.0);
+  const int q = (int)((long long)k & 3);
+  const double u = q & 1 ? c : s, v = q & 1 ? s : c;
+  return double2{q == 1 || q == 2 ? -v : v, q & 2 ? -u : u};  // cos, sin
 }
 
 struct Kv4Append {
   const void* qkv;
   int splits, W, nq, nkv;
   int v_wgs, v_chunks, v_units;  // the first workgroups: V, v_units units of a wave each, v_chunks per 4 positions
-  int chunks, heads_per_wg;      // the others: queries and keys of a row
+  int chunks, units_per_wg;      // the others: queries and keys of a row, chunks each
   int64_t slice;
   const uint16_t *q_norm, *k_norm, *v_norm;
   float eps;
@@ -66,83 +68,122 @@ struct Kv4Append {
   float x_k, x_eps;
 };
 
-// 8 dims of a head of a row: the sum of the projection's slices (slice order), or its bf16 values
+// 8 dims of a head of a row: the sum of the projection's slices, or its bf16 values
 template <int HD, bool F32>
-__device__ __forceinline__ void load8(const Kv4Append& a, int row, int head, int sub, float (&v)[8]) {
-  const int64_t off = ((int64_t)row * (a.nq + 2 * a.nkv) + head) * HD + sub * 8;
-  if constexpr (!F32) {
-    const u32x4 r = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(a.qkv) + off);
+struct Row8;
+template <int HD>
+struct Row8<HD, false> {
+  u32x4 r;
+  __device__ __forceinline__ void load(const Kv4Append& a, int row, int head, int sub) {
+    const int64_t off = ((int64_t)row * (a.nq + 2 * a.nkv) + head) * HD + sub * 8;
+    r = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(a.qkv) + off);
+  }
+  template <typename T>
+  __device__ __forceinline__ void values(float, T (&v)[8]) const {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      v[2 * e] = bits_f32(r[e] << 16);
-      v[2 * e + 1] = bits_f32(r[e] & 0xffff0000u);
-    }
-  } else {
-    const float* src = reinterpret_cast<const float*>(a.qkv) + off;
-    f32x4 s0 = *reinterpret_cast<const f32x4*>(src), s1 = *reinterpret_cast<const f32x4*>(src + 4);
-    for (int sp = 1; sp < a.splits; ++sp) {
-      s0 += *reinterpret_cast<const f32x4*>(src + sp * a.slice);
-      s1 += *reinterpret_cast<const f32x4*>(src + sp * a.slice + 4);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = s0[e];
-      v[4 + e] = s1[e];
+      v[2 * e] = (T)bits_f32(r[e] << 16);
+      v[2 * e + 1] = (T)bits_f32(r[e] & 0xffff0000u);
     }
   }
+};
+template <int HD>
+struct Row8<HD, true> {
+  double s[8];
+  __device__ __forceinline__ void load(const Kv4Append& a, int row, int head, int sub) {
+    const float* src = reinterpret_cast<const float*>(a.qkv) + ((int64_t)row * (a.nq + 2 * a.nkv) + head) * HD + sub * 8;
+    f32x4 x = *reinterpret_cast<const f32x4*>(src), y = *reinterpret_cast<const f32x4*>(src + 4);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = (double)(e < 4 ? x[e % 4] : y[e % 4]);
+    for (int sp = 1; sp < a.splits; ++sp) {
+      x = *reinterpret_cast<const f32x4*>(src + sp * a.slice);
+      y = *reinterpret_cast<const f32x4*>(src + sp * a.slice + 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += (double)(e < 4 ? x[e % 4] : y[e % 4]);
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void values(float scale, T (&v)[8]) const {  // times the row scale
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (T)(s[e] * (double)scale);
+  }
+};
+template <int L, typename T>
+__device__ __forceinline__ T lanes_sum(T x) {
+#pragma unroll
+  for (int o = 1; o < L; o <<= 1) x += __shfl_xor(x, o, 64);
+  return x;
 }
 // the row scale of a projection whose input is normed later: L lanes (each with its number sub) for one row
 template <int L>
 __device__ __forceinline__ float row_scale(const Kv4Append& a, int row, int sub) {
   float ss = 0.0f;
   for (int j = sub; j < a.x_tiles; j += L) ss += a.x_ssq[(int64_t)row * a.x_tiles + j];
-  return rsqrtf(row_sum<L>(ss) / a.x_k + a.x_eps);
+  return rsqrtf(lanes_sum<L>(ss) / a.x_k + a.x_eps);
 }
 // v * rsqrt(mean(v^2) + eps) * w of a head in HD / 8 lanes
-template <int HD>
-__device__ __forceinline__ void norm8(const Kv4Append& a, const uint16_t* w, int sub, float (&v)[8]) {
-  float ss = 0.0f;
+template <int HD, typename T>
+__device__ __forceinline__ void norm8(const Kv4Append& a, const uint16_t* w, int sub, T (&v)[8]) {
+  T ss = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
-  ss = row_sum<HD / 8>(ss);
+  ss = lanes_sum<HD / 8>(ss);
   if (!w) return;
-  const float r = rsqrtf(ss / (float)HD + a.eps);
+  T r;
+  if constexpr (sizeof(T) == 8) r = rsqrt(ss * (1.0 / HD) + (double)a.eps);
+  else r = rsqrtf(ss / (float)HD + a.eps);
   const u32x4 g = *reinterpret_cast<const u32x4*>(w + sub * 8);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    v[2 * e] = v[2 * e] * r * bits_f32(g[e] << 16);
-    v[2 * e + 1] = v[2 * e + 1] * r * bits_f32(g[e] & 0xffff0000u);
+    v[2 * e] = v[2 * e] * r * (T)bits_f32(g[e] << 16);
+    v[2 * e + 1] = v[2 * e + 1] * r * (T)bits_f32(g[e] & 0xffff0000u);
   }
 }
+// to bf16 by way of float32, as a cache's words are formed from float32 rows (the compiler would round once)
+template <typename T>
+__device__ __forceinline__ uint16_t round16(T x) {
+  float f = (float)x;
+  asm("" : "+v"(f));
+  return f32_to_bf16(f);
+}
 // the codes of 8 dims, half byte e dim e, and the scale and offset of their 64 (8 lanes; every lane runs this)
-__device__ __forceinline__ uint32_t codes8(const float (&v)[8], uint32_t& sb) {
-  float lo = v[0], hi = v[0];
+template <typename T>
+__device__ __forceinline__ uint32_t codes8(const T (&v)[8], uint32_t& sb) {
+  T lo = v[0], hi = v[0];
 #pragma unroll
   for (int e = 1; e < 8; ++e) {
-    lo = fminf(lo, v[e]);
-    hi = fmaxf(hi, v[e]);
+    lo = fmin(lo, v[e]);
+    hi = fmax(hi, v[e]);
   }
 #pragma unroll
   for (int m = 1; m < 8; m <<= 1) {
-    lo = fminf(lo, __shfl_xor(lo, m, 64));
-    hi = fmaxf(hi, __shfl_xor(hi, m, 64));
+    lo = fmin(lo, __shfl_xor(lo, m, 64));
+    hi = fmax(hi, __shfl_xor(hi, m, 64));
   }
-  uint16_t s16 = f32_to_bf16((hi - lo) / 15.0f);
+  uint16_t s16 = round16(sizeof(T) == 8 ? (hi - lo) * (T)(1.0 / 15.0) : (hi - lo) / (T)15);
   if (!(bf16_to_f32(s16) > 0.0f)) s16 = 0x3f80;
-  const uint16_t b16 = f32_to_bf16(lo);
-  const float sf = bf16_to_f32(s16), bf = bf16_to_f32(b16);
+  const uint16_t b16 = round16(lo);
+  const T s = (T)bf16_to_f32(s16), b = (T)bf16_to_f32(b16);
   sb = (uint32_t)s16 | ((uint32_t)b16 << 16);
+  // 64 bits: a product with the reciprocal, off by 2^-47 (one step from a float32 one; of 15 steps: 1e-13)
+  const T r0 = (T)(1.0f / (float)s), inv = r0 * ((T)2 - s * r0);
   uint32_t cw = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) cw |= (uint32_t)(int)fminf(fmaxf(rintf((v[e] - bf) / sf), 0.0f), 15.0f) << (4 * e);
+  for (int e = 0; e < 8; ++e) {
+    T q;
+    if constexpr (sizeof(T) == 8) q = rint((v[e] - b) * inv);
+    else q = rintf((v[e] - b) / s);
+    cw |= (uint32_t)(int)fmin(fmax(q, (T)0), (T)15) << (4 * e);
+  }
   return cw;
 }
 
 // V of 4 positions (a multiple of 4 and the next) of row b: a wave has NT of them side by side, L lanes each,
 // so that bytes of neighbouring tokens, which lie together, are written as words (2048 tokens, 8 heads of 128 with
-// 32 query heads: 19 us with queries, keys and values a byte at a time, 14.5 so). Other tokens stay as they are.
+// 32 query heads: 19 us with queries and keys when V went byte by byte, 14.5 so). Other tokens stay as they are.
 template <int HD, bool F32>
 __device__ __forceinline__ void append_v(const Kv4Append& a, int wg) {
+  using T = std::conditional_t<F32, double, float>;
   constexpr int L = HD / 8, NT = 64 / L, kParts = 4 / NT;  // a head's 4 tokens take kParts units of a wave
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, sub = lane % L, t = lane / L;
   const int quads = (a.W + 6) / 4, group = wg / a.v_chunks, chunk = wg - group * a.v_chunks;
@@ -156,14 +197,12 @@ __device__ __forceinline__ void append_v(const Kv4Append& a, int wg) {
     const int64_t pos64 = base + t0 + t;
     const bool stored = pos64 >= start && pos64 < start + a.W && pos64 >= 0 && pos64 < (int64_t)a.max_pages * a.page;
     const int row = b * a.W + (int)min(max(pos64 - start, (int64_t)0), (int64_t)a.W - 1), pos = stored ? (int)pos64 : 0;
-    float v[8];
-    load8<HD, F32>(a, row, a.nq + a.nkv + head, sub, v);
-    if (F32 && a.x_ssq) {
-      if (row != last) scale = row_scale<L>(a, row, sub);
-      last = row;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= scale;
-    }
+    Row8<HD, F32> x;
+    x.load(a, row, a.nq + a.nkv + head, sub);
+    if (F32 && a.x_ssq && row != last) scale = row_scale<L>(a, row, sub);
+    last = row;
+    T v[8];
+    x.values(scale, v);
     norm8<HD>(a, a.v_norm, sub, v);
     uint32_t sb;
     const uint32_t cw = codes8(v, sb), pw = __shfl_xor(cw, 2, 64);  // the dims 16 on (or back): the other half bytes
@@ -202,57 +241,72 @@ __device__ __forceinline__ void append_v(const Kv4Append& a, int wg) {
 
 template <int HD, bool F32>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Append a) {
-  constexpr int L = HD / 8, HPW = 64 / L;  // lanes per head, heads per wave
-  __shared__ float2 cs[HD / 2];
+  constexpr int L = HD / 8, HPW = 64 / L;  // lanes per head, heads per unit of a wave
+  __shared__ double2 cs[HD / 2];   // cosine, sine
+  __shared__ float2 csf[HD / 2];
   if ((int)blockIdx.x < a.v_wgs) {
     append_v<HD, F32>(a, blockIdx.x);
     return;
   }
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, sub = lane % L;
-  const int wg = blockIdx.x - a.v_wgs, row = wg / a.chunks, b = row / a.W, nheads = a.nq + a.nkv;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sub = lane % L;
+  const int wg = blockIdx.x - a.v_wgs, row = wg / a.chunks, b = row / a.W;
   const int64_t pos64 = (int64_t)a.seq_lens[b] + row % a.W + a.pos_offset;
   const bool stored = pos64 >= 0 && pos64 < (int64_t)a.max_pages * a.page;  // beyond the row's block table: dropped
   const int pos = stored ? (int)pos64 : 0;
   const int64_t pg = a.block_table[(int64_t)b * a.max_pages + pos / a.page];
   const int slot = pos % a.page;
-  const int h0 = (wg - row * a.chunks) * a.heads_per_wg, h1 = min(nheads, h0 + a.heads_per_wg);
-  int head = h0 + wv * HPW + lane / L;
-  float nxt[8];
-  load8<HD, F32>(a, row, min(head, nheads - 1), sub, nxt);  // in flight while the angles are reduced
+  const int q_units = (a.nq + HPW - 1) / HPW, units = q_units + (a.nkv + HPW - 1) / HPW;
+  const int u0 = (wg - row * a.chunks) * a.units_per_wg, u1 = min(units, u0 + a.units_per_wg);
+  // the head of a unit's lane, and the row's head that it reads (where heads do not fill a unit: the last one)
+  auto head_of = [&](int u) { return (u < q_units ? u : u - q_units) * HPW + lane / L; };
+  auto load = [&](int u, Row8<HD, F32>& x) {
+    x.load(a, row, u < q_units ? min(head_of(u), a.nq - 1) : a.nq + min(head_of(u), a.nkv - 1), sub);
+  };
+  int u = u0 + wv;
+  Row8<HD, F32> nxt;
+  load(min(u, units - 1), nxt);  // in flight while the angles are reduced
   const float scale = F32 && a.x_ssq ? row_scale<64>(a, row, lane) : 1.0f;
   for (int d = threadIdx.x; d < HD / 2; d += 256) {
-    float sn, c;
-    rope_exact((float)pos64, a.inv_freq[d], sn, c);
-    cs[d] = float2{c, sn};
+    cs[d] = rope_angle((double)pos64, a.inv_freq[d]);
+    csf[d] = float2{(float)cs[d].x, (float)cs[d].y};
   }
   __syncthreads();
   const bool first_half = sub < L / 2;
   const int d0 = (first_half ? sub : sub - L / 2) * 8;
-  for (; head - lane / L < h1; head += 4 * HPW) {  // whole waves: the shuffles below need every lane
-    float v[8];
+  for (; u < u1; u += 4) {
+    const Row8<HD, F32> x = nxt;
+    if (u + 4 < u1) load(u + 4, nxt);
+    const int head = head_of(u);
+    if (u < q_units) {
+      float v[8];
+      x.values(scale, v);
+      norm8<HD>(a, a.q_norm, sub, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = nxt[e] * scale;
-    if (head - lane / L + 4 * HPW < h1) load8<HD, F32>(a, row, min(head + 4 * HPW, nheads - 1), sub, nxt);
-    const bool is_q = head < a.nq;
-    norm8<HD>(a, is_q ? a.q_norm : a.k_norm, sub, v);
+      for (int e = 0; e < 8; ++e) {  // dim d pairs with d + HD / 2, L / 2 lanes away
+        const float partner = __shfl_xor(v[e], L / 2, 64);
+        const float2 t = csf[d0 + e];
+        v[e] = v[e] * t.x + (first_half ? -partner : partner) * t.y;
+      }
+      if (head < a.nq)
+        *reinterpret_cast<u32x4*>(a.q_out + ((int64_t)row * a.nq + head) * HD + sub * 8) =
+            u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+    } else {
+      double v[8];
+      x.values(scale, v);
+      norm8<HD>(a, a.k_norm, sub, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {  // dim d pairs with d + HD / 2, L / 2 lanes away
-#pragma clang fp contract(off)
-      const float partner = __shfl_xor(v[e], L / 2, 64);
-      const float2 t = cs[d0 + e];
-      const float x = v[e] * t.x, y = partner * t.y;
-      v[e] = first_half ? x - y : x + y;
+      for (int e = 0; e < 8; ++e) {
+        const double partner = __shfl_xor(v[e], L / 2, 64);
+        const double2 t = cs[d0 + e];
+        v[e] = v[e] * t.x + (first_half ? -partner : partner) * t.y;
+      }
+      uint32_t sb;
+      const uint32_t cw = codes8(v, sb);
+      if (!stored || head >= a.nkv) continue;
+      const int64_t at = (pg * a.nkv + head) * a.page + slot;
+      if (sub % 8 == 0) a.k_sb[at * (HD / 64) + sub / 8] = sb;
+      *reinterpret_cast<uint32_t*>(a.k_pool + at * (HD / 2) + kv4_k_word(sub)) = cw;
     }
-    if (is_q && head < h1)
-      *reinterpret_cast<u32x4*>(a.q_out + ((int64_t)row * a.nq + head) * HD + sub * 8) =
-          u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
-    if (__all(is_q)) continue;
-    uint32_t sb;
-    const uint32_t cw = codes8(v, sb);  // a wave may hold query and K heads, so every lane runs it
-    if (is_q || !stored || head >= h1) continue;
-    const int64_t at = (pg * a.nkv + head - a.nq) * a.page + slot;
-    if (sub % 8 == 0) a.k_sb[at * (HD / 64) + sub / 8] = sb;
-    *reinterpret_cast<uint32_t*>(a.k_pool + at * (HD / 2) + kv4_k_word(sub)) = cw;
   }
 }
 
@@ -268,14 +322,16 @@ int kv4_append(const void* qkv, int splits, int B, int W, int nq, int nkv, int h
   DSK_REQUIRE(((((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)v_norm) & 15) |
                (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15)) == 0, "%s: pointers must be 16-byte aligned", who);
   const int64_t rows = (int64_t)B * W;
-  const int heads = nq + nkv, per = hd == 128 ? 16 : 8;  // query and K heads of one pass of a workgroup's four waves
+  const int per_unit = hd == 128 ? 4 : 2;  // heads of a wave
+  const int64_t qk_units = ceil_div(nq, per_unit) + ceil_div(nkv, per_unit);
   DSK_REQUIRE(rows <= 0x7fffffff, "%s: %lld rows", who, (long long)rows);
-  // few rows: a workgroup per 16 (8) heads, so that the chip has work; many: one per row
-  const int heads_per_wg = rows < 256 ? per : (int)ceil_div(heads, per) * per, chunks = (int)ceil_div(heads, heads_per_wg);
+  // few rows: one unit per wave, so that the chip has work; many: a workgroup per row, which finds the angles once
+  // (2048 rows of 40 heads, before V went apart: 18.4 us, 20.3 with a unit per wave)
+  const int units_per_wg = rows < 256 ? 4 : (int)qk_units, chunks = (int)ceil_div(qk_units, units_per_wg);
   const int units = nkv * (hd / 128), v_units = rows < 256 ? 4 : units, v_chunks = (int)ceil_div(units, v_units);
   const int64_t v_wgs = (int64_t)B * ((W + 6) / 4) * v_chunks;
   DSK_REQUIRE(v_wgs + rows * chunks <= 0x7fffffff, "%s: %lld rows", who, (long long)rows);
-  Kv4Append a = {qkv, splits, W, nq, nkv, (int)v_wgs, v_chunks, v_units, chunks, heads_per_wg, rows * (nq + 2 * nkv) * hd,
+  Kv4Append a = {qkv, splits, W, nq, nkv, (int)v_wgs, v_chunks, v_units, chunks, units_per_wg, rows * (nq + 2 * nkv) * hd,
                  q_norm, k_norm, v_norm, eps, inv_freq, seq_lens, pos_offset, block_table, max_pages, page, (uint8_t*)k_pool,
                  (uint8_t*)v_pool, k_sb, v_sb, q_out, x_ssq, x_tiles, (float)(x_tiles * 16), x_eps};
   const dim3 grid((unsigned)(v_wgs + rows * chunks)), blk(256);
