@@ -267,8 +267,9 @@ int dsk_qkv_norm_rope_append(const void* qkv, int qkv_splits, int B, int W, int 
                              uint32_t* k_sb, uint32_t* v_sb, uint16_t* q_out, dsk_stream_t stream);
 
 /* Both append entries above write a DSK_KV_U4 pool too (head_dim 128 or 256, 16-byte aligned buffers):
- * a row then stays float32 from the projection's sum to its code, and is rotated by the exact product
- * of position and frequency. Tokens at positions beyond the row's block table are dropped.
+ * slices are then summed and keys normed, rotated (by the exact product of position and frequency) and
+ * quantised in 64 bits, so a code is the nearest to its value. Tokens at positions beyond the row's block
+ * table are dropped. Values up to 1e31 in magnitude read back as given; a group of wider ones does not.
  *
  * dsk_kv_read: positions first[b] + offset + i (i < n) of every row as bf16 rows k_out, v_out
  * [B, n, nkv, hd], whatever the cache holds them in: the values attention reads (mx.dequantize of a
@@ -340,11 +341,12 @@ int dsk_attention_rows(const uint16_t* q, int B, int W, int nq, int nkv, int hd,
  * the chip (a batch's rows by their lengths, read on the device) and join the splits in a second kernel;
  * prompts run in blocks of query rows. k and v of quantised caches are the values dsk_kv_read returns;
  * scores, softmax statistics and outputs stay float32, a probability enters P.V as p_terms bf16 terms: 3
- * (within 2^-26), or for W > 64 also 2 (2^-17, as dsk_attention's many-query form). What stands in a masked key, or in the slots behind the last one, never reaches the
- * output, infinities and NaN included; a row that sees no key becomes zeros. softcap as dsk_attention.
+ * (within 2^-26), or for W > 64 also 2 (2^-17, as dsk_attention's many-query form). What stands in a
+ * masked key, or in the slots behind the last one, never reaches the output, infinities and NaN included;
+ * a row that sees no key becomes zeros. softcap as dsk_attention.
  * head_dim 128 or 256, pages of a multiple of 32 tokens, scale > 0, 16-byte aligned buffers. max_ctx
  * bounds seq_lens[b] + W and sizes the grid (graph-stable). workspace:
- * dsk_attention_sinks_ws_bytes(...) bytes, 0 where none is used; no state is kept in it between calls,
+ * dsk_attention_sinks_ws_bytes(...) bytes (enough for every kv_dtype), 0 where none is used; no state is kept in it between calls,
  * calls that overlap need one each (DSK_ENOWS when it is too small). */
 size_t dsk_attention_sinks_ws_bytes(int B, int W, int nq, int nkv, int hd, int causal, int window,
                                     int sinks, int max_ctx);

@@ -38,7 +38,9 @@ def _require_cuda(*ts):
 
 def _on_device(t: torch.Tensor) -> None:
     """A kernel runs on the current device's current stream: refuse tensors of another device."""
-    if t.device.index not in (None, torch.cuda.current_device()):
+    if not t.is_cuda:
+        raise ValueError("dspark kernels need device tensors (got a CPU tensor)")
+    if t.device.index != torch.cuda.current_device():
         raise ValueError(f"tensors are on {t.device}, the current device is {torch.cuda.current_device()}: call under "
                          f"torch.cuda.device({t.device.index})")
 
@@ -480,18 +482,19 @@ def qkv_rope_append(qkv, B, W, nq, nkv, hd, q_norm, k_norm, eps, inv_freq, seq_l
     if q_out is None and nq:
         q_out = torch.empty((B * W, nq * hd), dtype=torch.bfloat16, device=qkv.device)
     if kv_dtype == DSK_KV_U4:   # 16-byte loads only
+        _on_device(qkv)
         qkv, q_norm, k_norm, v_norm = (t if t is None or t.data_ptr() % 16 == 0 else t.clone()
                                        for t in (qkv, q_norm, k_norm, v_norm))
     if x is not None and x.ssq is not None:
         if pos_offset or v_norm is not None:
             raise ValueError("qkv_rope_append: a normed-later input takes no pos_offset / v_norm")
-        call("dsk_qkv_rope_append_rn", ptr(qkv), splits, B, W, nq, nkv, hd, ptr(q_norm), ptr(k_norm), float(eps),
-             ptr(inv_freq), ptr(seq_lens), ptr(block_table), block_table.shape[1], page, kv_dtype, ptr(k_pool),
-             ptr(v_pool), ptr(k_sb), ptr(v_sb), ptr(q_out), ptr(x.ssq), x.K // 16, float(x.eps), stream_ptr())
+        call("dsk_qkv_rope_append_rn", addr(qkv), splits, B, W, nq, nkv, hd, addr(q_norm), addr(k_norm), float(eps),
+             addr(inv_freq), addr(seq_lens), addr(block_table), block_table.shape[1], page, kv_dtype, addr(k_pool),
+             addr(v_pool), addr(k_sb), addr(v_sb), addr(q_out), addr(x.ssq), x.K // 16, float(x.eps), stream_ptr())
         return q_out
-    call("dsk_qkv_norm_rope_append", ptr(qkv), splits, B, W, nq, nkv, hd, ptr(q_norm), ptr(k_norm), ptr(v_norm),
-         float(eps), ptr(inv_freq), ptr(seq_lens), int(pos_offset), ptr(block_table), block_table.shape[1], page,
-         kv_dtype, ptr(k_pool), ptr(v_pool), ptr(k_sb), ptr(v_sb), ptr(q_out), stream_ptr())
+    call("dsk_qkv_norm_rope_append", addr(qkv), splits, B, W, nq, nkv, hd, addr(q_norm), addr(k_norm), addr(v_norm),
+         float(eps), addr(inv_freq), addr(seq_lens), int(pos_offset), addr(block_table), block_table.shape[1], page,
+         kv_dtype, addr(k_pool), addr(v_pool), addr(k_sb), addr(v_sb), addr(q_out), stream_ptr())
     return q_out
 
 
@@ -501,7 +504,8 @@ def kv_read(first, n, nkv, hd, block_table, page, kv_dtype, k_pool, v_pool, k_sb
     (k, v) [B, n, nkv, hd], whatever the cache holds them in: the values attention reads. Positions outside
     the block table leave their rows of k_out / v_out as they were (unset without them)."""
     B = block_table.shape[0]
-    _require_cuda(first, k_pool)
+    if not (k_pool.is_contiguous() and v_pool.is_contiguous() and block_table.is_contiguous()):
+        raise ValueError("kv_read: pools and block_table must be contiguous")
     if first.dtype != torch.int32 or first.numel() != B or not first.is_contiguous():
         raise ValueError(f"kv_read: first must be int32 [{B}]")
     outs = []
@@ -513,6 +517,7 @@ def kv_read(first, n, nkv, hd, block_table, page, kv_dtype, k_pool, v_pool, k_sb
         outs.append(t)
     if n == 0:
         return tuple(outs)
+    _require_cuda(first, block_table)
     _on_device(k_pool)
     call("dsk_kv_read", addr(first), offset, B, n, nkv, hd, addr(block_table), block_table.shape[1], page, kv_dtype,
          addr(k_pool), addr(v_pool), addr(k_sb), addr(v_sb), addr(outs[0]), addr(outs[1]), stream_ptr())
@@ -528,6 +533,8 @@ def _attention_sinks(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table
                      v_sb, causal, window, softcap, sinks, out, p_terms):
     """dsk_attention_sinks into out (bf16 rows or a Packed)."""
     _on_device(q)
+    if k_pool.device != q.device or not k_pool.is_contiguous() or not v_pool.is_contiguous():
+        raise ValueError(f"attention: the pools must be contiguous, on {q.device}")
     packed = isinstance(out, Packed)
     odata = out.data if packed else out
     if q.dtype != torch.bfloat16 or not q.is_contiguous() or q.numel() != B * W * nq * hd:

@@ -82,3 +82,25 @@ def test_attention_workspace_too_small():
         rc, msg = _attend(max_ctx=4096, max_pages=64, ws=ws, wsb=n)
         assert rc == -4 and "workspace" in msg
     assert _hip.lib.dsk_attention_sinks_ws_bytes(1, 1, 4, 2, 64, 1, 0, 0, 4096) == 0
+
+
+def test_python_refusals():
+    """Host tensors, strided pools and lists of the wrong type, before anything is launched."""
+    import torch
+    from mlx_dspark import ops
+
+    table, lens = torch.zeros((1, 2), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    pool, sb = torch.zeros((2, 2, 64, 64), dtype=torch.uint8), torch.zeros((2, 2, 64, 2), dtype=torch.int32)
+    q = torch.zeros((1, 512), dtype=torch.bfloat16)
+    att = lambda **kw: ops.attention(q, 1, 1, 4, 2, 128, 0.1, lens, 64, table, 64, ops.DSK_KV_U4, pool, pool, sb, sb, **kw)
+    for call in (att, lambda: ops.kv_read(lens, 3, 2, 128, table, 64, ops.DSK_KV_U4, pool, pool, sb, sb),
+                 lambda: ops.qkv_rope_append(torch.zeros((1, 1024), dtype=torch.bfloat16), 1, 1, 4, 2, 128, None, None, 1e-6,
+                                             torch.zeros(64), lens, table, 64, ops.DSK_KV_U4, pool, pool, sb, sb)):
+        with pytest.raises(ValueError, match="device tensors"):
+            call()
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.kv_read(lens, 3, 2, 128, table, 64, ops.DSK_KV_U4, pool[:, :, ::2], pool, sb, sb)
+    with pytest.raises(ValueError, match="int32"):
+        ops.kv_read(lens.long(), 3, 2, 128, table, 64, ops.DSK_KV_U4, pool, pool, sb, sb)
+    k, v = ops.kv_read(lens, 0, 2, 128, table, 64, ops.DSK_KV_U4, pool, pool, sb, sb)   # nothing to read
+    assert k.shape == v.shape == (1, 0, 2, 128)
