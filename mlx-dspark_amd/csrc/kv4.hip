@@ -348,7 +348,8 @@ int kv4_append(const void* qkv, int splits, int B, int W, int nq, int nkv, int h
 
 // ----------------------------------------------------------------------------- read back
 // K and V of positions first[b] + offset + i, i < n, as bf16 rows: one workgroup per 32 positions (whole
-// V blocks) of a (row, kv head), 8 dims per thread and step. A copy: bound by the bytes it writes.
+// V blocks) of a (row, kv head), 8 dims per thread and step. A copy: bound by the bytes it writes (4-bit codes of
+// 32768 tokens, 8 heads of 128: 29.6 us, 5.8 TB/s read and written; of 1027, 256 dims: 7 us, its chain of loads).
 struct KvRead {
   const int32_t* first;
   int offset, n, nkv;
