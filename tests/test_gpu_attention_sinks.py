@@ -345,3 +345,51 @@ def test_non_default_stream(dev):
     with torch.cuda.stream(s):
         got = run(dev, c, q, [100], 3, 4, 2)
     assert torch.equal(got, base)
+
+
+@pytest.mark.parametrize("bits,window,sinks,W", [(4, 0, 0, 1), (4, 0, 0, 90), (8, 100, 4, 9), (0, 100, 4, 1)])
+def test_pages_past_32_bit_offsets(dev, bits, window, sinks, W):
+    """The same pages at the end of pools of more than 4 GiB: append, attention and read-back bit for bit."""
+    from mlx_dspark import ops
+
+    nq, nkv, hd, page, n = 8, 2, 128, 64, 300
+    kv = {0: ops.DSK_KV_BF16, 8: ops.DSK_KV_U8, 4: ops.DSK_KV_U4}[bits]
+    width, dt = (hd // 2 if bits == 4 else hd), (torch.uint8 if bits else torch.bfloat16)
+    far = (2 ** 32 + 2 ** 20) // (nkv * page * width * (1 if bits else 2))
+    need = -(-(n + W) // page)
+    inv = ops.rope_inv_freq(hd, 1e6, dev)
+    x = torch.randn((1, n + W, (nq + 2 * nkv) * hd), generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).to(dev)
+    outs = []
+    for first in (0, far):
+        print(f"far bits={bits} W={W} first page {first}", flush=True)
+        table = (first + torch.randperm(need, generator=torch.Generator().manual_seed(1))).to(torch.int32)[None].to(dev)
+        pools = [torch.empty((first + need, nkv, page, width), dtype=dt, device=dev) for _ in range(2)]
+        sbs = [torch.empty((first + need, nkv, page, hd // 64), dtype=torch.int32, device=dev) if bits else None for _ in range(2)]
+        cache = (table, page, kv, *pools, *sbs)
+        sl = torch.zeros(1, dtype=torch.int32, device=dev)
+        ops.qkv_rope_append(x[0, :n].contiguous(), 1, n, nq, nkv, hd, None, None, 1e-6, inv, sl, *cache)
+        sl.fill_(n)
+        q = ops.qkv_rope_append(x[0, n:].contiguous(), 1, W, nq, nkv, hd, None, None, 1e-6, inv, sl, *cache)
+        o = ops.attention(q, 1, W, nq, nkv, hd, hd ** -0.5, sl, n + W, *cache, window=window, sinks=sinks)
+        k, v = ops.kv_read(torch.zeros(1, dtype=torch.int32, device=dev), n + W, nkv, hd, *cache)
+        outs.append([t.cpu() for t in (q, o, k, v)])
+        del pools, sbs, cache
+    torch.cuda.empty_cache()
+    assert all(torch.equal(a, b) for a, b in zip(*outs)) and all(t.float().abs().sum() > 0 for t in outs[0])
+
+
+@pytest.mark.parametrize("bits,hd,nq,nkv,W,window,sinks", [
+    (4, 128, 8, 2, 1, 0, 0), (4, 256, 4, 2, 20, 0, 0),
+    *((bits, 128, 8, 2, W, window, sinks) for bits in (4, 0) for W, window, sinks in ((9, 40, 70), (100, 30, 4)))])
+def test_table_entries_that_no_query_sees(dev, bits, hd, nq, nkv, W, window, sinks):
+    """Table entries behind the rows' last pages, and the window's expired ones, may hold anything: here pages
+    of another row."""
+    lens = [150, 3]
+    c = Cache(bits, 2, nkv, hd, 6, 64, seed=7)
+    q = queries(2, W, nq, hd, 5)
+    want, tol = reference(c, q, lens, W, nq, nkv, True, window, sinks, hd ** -0.5)
+    for b, n in enumerate(lens):
+        seen = {int(j) // 64 for j in torch.nonzero(visible(n, W, n + W, True, window, sinks).any(0)).view(-1)}
+        for p in set(range(6)) - seen:
+            c.table[b, p] = 0
+    check(run(dev, c, q, lens, W, nq, nkv, True, window, sinks, rows=W > 64), want, tol)
