@@ -15,8 +15,8 @@
 // range and nothing is lost, and a block costs one vote instead of two lane exchanges and a rescale.
 //
 // Measured, us (the kernel, then with the join of its splits in a graph; rates are of the whole):
-//   4-bit, 32 heads of 128 over 8: one token after 16384 .. 65536 in 4 rows 46, 54: 3.2 TB/s of codes; 16 tokens
-//     after 4096 11.7, 16; a prompt of 4096 tokens 268, unsplit: 0.51 PFLOP/s of scores and outputs, 1.03 with the
+//   4-bit, 32 heads of 128 over 8: one token after 16384 .. 65536 in 4 rows 46, 52: 3.3 TB/s of codes; 16 tokens
+//     after 4096 11.7, 15.5; a prompt of 4096 tokens 268, unsplit: 0.51 PFLOP/s of scores and outputs, 1.03 with the
 //     three terms
 //   8-bit, window 4096 and 64 sinks, one token in 8 rows of 2048 .. 32768 20, 24: 2.7 TB/s
 //   bf16, 16 heads of 256 over 8, window 1024, 9 tokens 12.4, 16
@@ -68,6 +68,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kSplitUnit = 4;       // splits are multiples of this many 32-key blocks: one per wave, or two chunks of 64
 constexpr float kMaxSlack = 8.0f;   // how far (log2) a score may pass the running maximum
 constexpr int kDecodeMaxW = 64;      // new tokens per row of a decode or verify pass
+constexpr int kSpreadRows = 5;      // query rows whose three terms fit the 16 columns of a tile
 constexpr int kBalancedRows = 64;   // rows whose lengths a workgroup reads to place its split, one per lane
 
 // The 32-key blocks that query tokens i0 .. i1 of row b look at.
@@ -273,6 +274,21 @@ struct Tile {
       for (int k = 0; k < kTerms; ++k) t[k][i] = w[k];
     }
   }
+  // of 8 probabilities the term that the lane's column takes (kTerms 1): k1, k2 are 1 from the second and third on
+  static __device__ __forceinline__ void own_term(const f32x4& a, const f32x4& b, float k1, float k2, u32x4& t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4& s = i < 2 ? a : b;
+      float x = s[2 * (i & 1)], y = s[2 * (i & 1) + 1];
+      uint32_t w = pack_bf16x2(x, y);
+      x = fmaf(-k1, bits_f32(w << 16), x);
+      y = fmaf(-k1, bits_f32(w & 0xffff0000u), y);
+      w = pack_bf16x2(x, y);
+      x = fmaf(-k2, bits_f32(w << 16), x);
+      y = fmaf(-k2, bits_f32(w & 0xffff0000u), y);
+      t[i] = pack_bf16x2(x, y);
+    }
+  }
   // O^T += V^T . P^T for d tiles D .. D + 3 and a block's 32 keys, term by term: four independent products
   // between two on the same accumulator.
   template <int D>
@@ -332,8 +348,15 @@ __device__ __forceinline__ void add_nonfinite(const SinkArgs& a, Tile<HD, TERMS>
         const uint32_t w = e < 4 ? (e < 2 ? t[u][i][0] : t[u][i][1]) : (e < 6 ? t[u][i][2] : t[u][i][3]);
         p[u] += bits_f32((w << (e & 1 ? 0 : 16)) & 0xffff0000u);
       }
-      p[u] = __shfl(p[u], from, 64);
       vis[u] = see[u].sees(base + k);
+      if constexpr (TERMS == 1) {  // the terms are in three columns: all of them to the first
+        const int c = (lane & 15) % kSpreadRows + (from & 48);
+        const float t0 = __shfl(p[u], c, 64), t1 = __shfl(p[u], c + kSpreadRows, 64), t2 = __shfl(p[u], c + 2 * kSpreadRows, 64);
+        p[u] = t0 + t1 + t2;
+        vis[u] = bool((int)vis[u] & (int)((lane & 15) < kSpreadRows));
+      } else {
+        p[u] = __shfl(p[u], from, 64);
+      }
     }
 #pragma unroll
     for (int d = 0; d < HD / 16; ++d)
@@ -603,7 +626,11 @@ __device__ __forceinline__ u32x4 v_operand(const uint8_t* blk, int d, int lane) 
 // two); the others would spill.
 template <int HD, int KVT> constexpr int kTileWaves = HD == 128 || KVT == DSK_KV_U4 ? 2 : 1;
 
-template <int HD, int KVT>
+// SPREAD, for up to 5 rows: each stands in three columns, which compute the same scores and each take another
+// term of the probabilities, so that one product in place of three adds them; the columns are summed at the end
+// (us, without / with: 4-bit, one token in 32 rows of 4096, 32 heads 51.4 / 48.1, in 4 rows of 16384 .. 65536
+// 56.5 / 54.9, in 8 rows of 8192, 16 heads of 256 50.0 / 47.1; 8-bit, window 4096, 8 rows 24.0 / 23.5).
+template <int HD, int KVT, bool SPREAD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<HD, KVT>, 2))) void attention_tile_kernel(SinkArgs a) {
   constexpr int KS = HD / 32, DT = HD / 16;
   constexpr int VC = KVT == DSK_KV_U8 ? 16 : 8, NI = HD / VC / 8;  // V items (4 keys x VC dims) per lane
@@ -615,7 +642,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<
   const SplitTask t = split_task(a, slot, group);
   if (t.live == 0) return;
   const KeyPlan& p = t.p;
-  const int r0 = group * a.grows, r = r0 + n, rc = min(r, a.R - 1);
+  const int r0 = group * a.grows, r = r0 + (SPREAD ? n % kSpreadRows : n), rc = min(r, a.R - 1);
+  const float k1 = n >= kSpreadRows ? 1.0f : 0.0f, k2 = n >= 2 * kSpreadRows ? 1.0f : 0.0f;
   const int ri = a.by_G.quot(rc);
   const int pos = p.off + ri, pos_lo = p.off + a.by_G.quot(r0), pos_hi = p.off + a.by_G.quot(min(r0 + 16, a.R) - 1);
   const float c2 = (a.softcap > 0.0f ? 1.0f : a.scale) * kLog2e;
@@ -652,8 +680,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(src + KRaw<HD, KVT>::dim(s, g));
   }
-  Tile<HD, 3> tiles[1];
-  Tile<HD, 3>& tile = tiles[0];
+  constexpr int kTerms = SPREAD ? 1 : 3;
+  Tile<HD, kTerms> tiles[1];
+  Tile<HD, kTerms>& tile = tiles[0];
   tile.clear();
   uint8_t* vlds = lds + wv * DT * kVTile;
   if (nblk > 0) {  // the loop within: around it, the count of loads in flight would have to hold for no loads too
@@ -688,8 +717,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<
       const float mx = tile.largest(st, c2);
       if (__any(tile.passes(mx))) tile.raise(mx);
       tile.soften(st[0], st[1], c2);
-      u32x4 pt[1][3];
-      Tile<HD, 3>::terms(st[0], st[1], pt[0]);
+      u32x4 pt[1][kTerms];
+      if constexpr (SPREAD) Tile<HD, kTerms>::own_term(st[0], st[1], k1, k2, pt[0][0]);
+      else Tile<HD, kTerms>::terms(st[0], st[1], pt[0]);
       bool bad = false;
       if constexpr (kRows) {
 #pragma unroll
@@ -737,7 +767,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<
     wq[w] = wml[w][n].x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(wml[w][n].x - M);
     L += wq[w] * wml[w][n].y;
   }
-  if (r >= a.R) return;
+  if (r >= a.R || (SPREAD && n >= kSpreadRows)) return;
   const bool whole = t.live == 1;
   const float inv = L != 0.0f ? 1.0f / L : 0.0f;  // no visible key: zeros; a NaN sum stays NaN
 #pragma unroll
@@ -746,7 +776,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<
     f32x4 s = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int w = 0; w < 4; ++w)
-      if (wq[w] != 0.0f) s += mo[(w * DT + d) * 64 + lane] * wq[w];
+      if (wq[w] != 0.0f) {
+        const f32x4* o = &mo[(w * DT + d) * 64 + lane];
+        s += (SPREAD ? o[0] + (o[kSpreadRows] + o[2 * kSpreadRows]) : o[0]) * wq[w];
+      }
     if (whole) {
       s *= inv;
       *reinterpret_cast<uint2*>(a.out + sink_out_index(a, HD, t.b, r, kvh, d * 16 + 4 * g)) =
@@ -1145,7 +1178,9 @@ template <int HD, int KVT>
 static void launch_sinks(const SinkArgs& a, const SinkPlan& s, int terms, hipStream_t st) {
   const dim3 grid((unsigned)(s.slots * a.nkv), (unsigned)s.groups);
   if (s.tile) {
-    hipLaunchKernelGGL((attention_tile_kernel<HD, KVT>), grid, dim3(256), 0, st, a);
+    constexpr bool kSpread = KVT != DSK_KV_BF16;  // bf16 waits for its loads and gains nothing
+    if (kSpread && a.R <= kSpreadRows) hipLaunchKernelGGL((attention_tile_kernel<HD, KVT, kSpread>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((attention_tile_kernel<HD, KVT, false>), grid, dim3(256), 0, st, a);
   } else if (s.waves == 8) {
     if constexpr (HD == 128) {
       if (terms == 2) hipLaunchKernelGGL((attention_block_kernel<HD, KVT, 8, 2, 2>), grid, dim3(512), 0, st, a);
