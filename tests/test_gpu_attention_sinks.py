@@ -197,7 +197,7 @@ def test_values_only_some_rows_see(dev, bits, hd, nq, nkv, W, n, window, sinks):
     check(run(dev, c, q, [n], W, nq, nkv, True, window, sinks, rows=W > 64), want, tol)
 
 
-@pytest.mark.parametrize("hd,nq,nkv,W", [(128, 4, 2, 5), (256, 4, 2, 9), (128, 8, 2, 70)])
+@pytest.mark.parametrize("hd,nq,nkv,W", [(128, 4, 2, 5), (256, 4, 2, 9), (128, 8, 2, 70), (128, 2, 2, 5)])
 def test_values_past_the_range_of_four_bits(dev, hd, nq, nkv, W):
     """A scale and offset that are finite, whose values are not (15 * 2^125 + 2^125), in the newest token: the
     rows before do not see it, the last one does (all its values are 2^125 or more)."""
@@ -345,6 +345,23 @@ def test_non_default_stream(dev):
     with torch.cuda.stream(s):
         got = run(dev, c, q, [100], 3, 4, 2)
     assert torch.equal(got, base)
+
+
+@pytest.mark.parametrize("bits,hd,nq,nkv,W,lens,window,sinks", [
+    (4, 128, 2, 2, 5, [70, 33], 0, 0), (4, 128, 8, 2, 1, [3000], 0, 0), (8, 128, 4, 2, 2, [300], 40, 4),
+    (4, 256, 3, 1, 1, [64, 95], 40, 1), (8, 256, 2, 2, 4, [129], 64, 33), (4, 128, 2, 2, 5, [500], 33, 3)])
+@pytest.mark.parametrize("poison", [False, True])
+def test_few_rows_in_columns(dev, bits, hd, nq, nkv, W, lens, window, sinks, poison):
+    """Up to five query rows per kv head, each in three columns; with an infinity or NaN in the newest token, which
+    only the last row sees, and in the first row's last windowed key."""
+    print(f"columns bits={bits} hd={hd} W={W} lens={lens} window={window} poison={poison}", flush=True)
+    c = Cache(bits, len(lens), nkv, hd, -(-(max(lens) + W) // 64), 64, seed=9)
+    if poison:
+        for b, n in enumerate(lens):
+            c.poison(b, torch.tensor([n + W - 1] + ([n - window + 1] if window else [])))
+    q = queries(len(lens), W, nq, hd, 1)
+    want, tol = reference(c, q, lens, W, nq, nkv, True, window, sinks, hd ** -0.5)
+    check(run(dev, c, q, lens, W, nq, nkv, True, window, sinks), want, tol)
 
 
 @pytest.mark.parametrize("bits,window,sinks,W", [(4, 0, 0, 1), (4, 0, 0, 90), (8, 100, 4, 9), (0, 100, 4, 1)])
