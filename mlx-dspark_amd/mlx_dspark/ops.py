@@ -36,13 +36,16 @@ def _require_cuda(*ts):
             raise ValueError("dspark kernels need device tensors (got a CPU tensor)")
 
 
-def _on_device(t: torch.Tensor) -> None:
-    """A kernel runs on the current device's current stream: refuse tensors of another device."""
-    if not t.is_cuda:
+def _stream_of(t: torch.Tensor) -> int:
+    """The current stream. A kernel runs on the current device's: tensors of another one are refused. (Integers
+    throughout: torch's device and stream objects would cost a call 3 us.)"""
+    i = t.get_device()
+    if i < 0:
         raise ValueError("dspark kernels need device tensors (got a CPU tensor)")
-    if t.device.index != torch.cuda.current_device():
+    if i != torch._C._cuda_getDevice():
         raise ValueError(f"tensors are on {t.device}, the current device is {torch.cuda.current_device()}: call under "
-                         f"torch.cuda.device({t.device.index})")
+                         f"torch.cuda.device({i})")
+    return torch._C._cuda_getCurrentRawStream(i)
 
 
 # ----------------------------------------------------------------------------- workspace
@@ -481,20 +484,23 @@ def qkv_rope_append(qkv, B, W, nq, nkv, hd, q_norm, k_norm, eps, inv_freq, seq_l
         qkv = qkv.contiguous().to(torch.bfloat16)
     if q_out is None and nq:
         q_out = torch.empty((B * W, nq * hd), dtype=torch.bfloat16, device=qkv.device)
-    if kv_dtype == DSK_KV_U4:   # 16-byte loads only
-        _on_device(qkv)
-        qkv, q_norm, k_norm, v_norm = (t if t is None or t.data_ptr() % 16 == 0 else t.clone()
-                                       for t in (qkv, q_norm, k_norm, v_norm))
+    if kv_dtype == DSK_KV_U4:
+        stream = _stream_of(qkv)
+        _require_cuda(seq_lens, block_table, inv_freq, k_pool, v_pool)
+        if ((addr(qkv) or 0) | (addr(q_norm) or 0) | (addr(k_norm) or 0) | (addr(v_norm) or 0)) & 15:   # 16-byte loads only
+            qkv, q_norm, k_norm, v_norm = (None if t is None else t.clone() for t in (qkv, q_norm, k_norm, v_norm))
+    else:
+        stream = stream_ptr()
     if x is not None and x.ssq is not None:
         if pos_offset or v_norm is not None:
             raise ValueError("qkv_rope_append: a normed-later input takes no pos_offset / v_norm")
         call("dsk_qkv_rope_append_rn", addr(qkv), splits, B, W, nq, nkv, hd, addr(q_norm), addr(k_norm), float(eps),
              addr(inv_freq), addr(seq_lens), addr(block_table), block_table.shape[1], page, kv_dtype, addr(k_pool),
-             addr(v_pool), addr(k_sb), addr(v_sb), addr(q_out), addr(x.ssq), x.K // 16, float(x.eps), stream_ptr())
+             addr(v_pool), addr(k_sb), addr(v_sb), addr(q_out), addr(x.ssq), x.K // 16, float(x.eps), stream)
         return q_out
     call("dsk_qkv_norm_rope_append", addr(qkv), splits, B, W, nq, nkv, hd, addr(q_norm), addr(k_norm), addr(v_norm),
          float(eps), addr(inv_freq), addr(seq_lens), int(pos_offset), addr(block_table), block_table.shape[1], page,
-         kv_dtype, addr(k_pool), addr(v_pool), addr(k_sb), addr(v_sb), addr(q_out), stream_ptr())
+         kv_dtype, addr(k_pool), addr(v_pool), addr(k_sb), addr(v_sb), addr(q_out), stream)
     return q_out
 
 
@@ -511,16 +517,16 @@ def kv_read(first, n, nkv, hd, block_table, page, kv_dtype, k_pool, v_pool, k_sb
     outs = []
     for t in (k_out, v_out):
         if t is None:
-            t = torch.empty((B, n, nkv, hd), dtype=torch.bfloat16, device=k_pool.device)
+            t = torch.empty_like(outs[0]) if outs else k_pool.new_empty((B, n, nkv, hd), dtype=torch.bfloat16)
         elif t.dtype != torch.bfloat16 or tuple(t.shape) != (B, n, nkv, hd) or not t.is_contiguous():
             raise ValueError(f"kv_read: outputs must be contiguous bf16 [{B}, {n}, {nkv}, {hd}]")
         outs.append(t)
     if n == 0:
         return tuple(outs)
-    _require_cuda(first, block_table)
-    _on_device(k_pool)
+    _require_cuda(first, block_table, *outs)
+    stream = _stream_of(k_pool)
     call("dsk_kv_read", addr(first), offset, B, n, nkv, hd, addr(block_table), block_table.shape[1], page, kv_dtype,
-         addr(k_pool), addr(v_pool), addr(k_sb), addr(v_sb), addr(outs[0]), addr(outs[1]), stream_ptr())
+         addr(k_pool), addr(v_pool), addr(k_sb), addr(v_sb), addr(outs[0]), addr(outs[1]), stream)
     return tuple(outs)
 
 
@@ -532,8 +538,8 @@ def _sinks_ws_bytes(*args) -> int:
 def _attention_sinks(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table, page, kv_dtype, k_pool, v_pool, k_sb,
                      v_sb, causal, window, softcap, sinks, out, p_terms):
     """dsk_attention_sinks into out (bf16 rows or a Packed)."""
-    _on_device(q)
-    if k_pool.device != q.device or not k_pool.is_contiguous() or not v_pool.is_contiguous():
+    stream = _stream_of(q)
+    if k_pool.get_device() != q.get_device() or not k_pool.is_contiguous() or not v_pool.is_contiguous():
         raise ValueError(f"attention: the pools must be contiguous, on {q.device}")
     packed = isinstance(out, Packed)
     odata = out.data if packed else out
@@ -544,13 +550,14 @@ def _attention_sinks(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table
     if seq_lens.dtype != torch.int32 or seq_lens.numel() != B or block_table.dtype != torch.int32 or \
             block_table.shape[0] != B or not (seq_lens.is_contiguous() and block_table.is_contiguous()):
         raise ValueError(f"attention: seq_lens and block_table must be contiguous int32 of {B} rows")
+    _require_cuda(seq_lens, block_table, v_pool, odata)
     args = (B, W, nq, nkv, hd, int(bool(causal)), int(window), int(sinks), int(max_ctx))
     need = _sinks_ws_bytes(*args)
     # per call: passes on two streams, or of two captured graphs, may overlap
-    buf = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    buf = q.new_empty(need // 2) if need else None   # bytes in pairs
     call("dsk_attention_sinks", addr(q), *args[:5], scale, *args[5:8], softcap, p_terms, addr(seq_lens), args[8],
          addr(block_table), block_table.shape[1], page, kv_dtype, addr(k_pool), addr(v_pool), addr(k_sb), addr(v_sb),
-         addr(odata), int(packed), addr(buf), need, stream_ptr())
+         addr(odata), int(packed), addr(buf), need, stream)
 
 
 def attention(q, B, W, nq, nkv, hd, scale, seq_lens, max_ctx, block_table, page, kv_dtype, k_pool,
