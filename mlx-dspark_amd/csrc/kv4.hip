@@ -10,10 +10,10 @@ namespace dsk {
 // q, k: x * rsqrt(mean(x^2) + eps) * w, rotated by pos * inv_freq; k and v to 4-bit codes (kv4.h). A row is not
 // rounded between its projection's sum and its code or its bf16 query: to bf16, that would move about one code
 // in a hundred. Keys are formed in 64 bits, and so are the sums of slices: in 32, a few of the codes of a
-// 2048-token prompt are not the nearest (15.9 us instead of 14.5 for 40 heads of 128 with 8 of V).
+// 2048-token prompt are not the nearest (1.4 us more for 40 heads of 128 with 8 of V).
 //
 // What bounds it: few rows, the chain of loads (lengths, row, angles: 6.6 us for one token in a graph, of which
-// about 4 are two launches); many, the bytes: 44 MB for that prompt, 2.8 TB/s.
+// about 4 are two launches); many, the bytes: 44 MB for that prompt, 14.4 us, 3.1 TB/s.
 //
 // Queries and keys: one workgroup per token row and chunk of heads; the row's HD / 2 sines and cosines are found
 // once, one per thread, for all heads of the chunk; then 8 dims per lane, HD / 8 lanes per head. V, in the same
@@ -52,6 +52,7 @@ struct Kv4Append {
   int splits, W, nq, nkv;
   int v_wgs, v_chunks, v_units;  // the first workgroups: V, v_units units of a wave each, v_chunks per 4 positions
   int chunks, units_per_wg;      // the others: queries and keys of a row, chunks each
+  int q_past;                    // queries are stored past the caches
   int64_t slice;
   const uint16_t *q_norm, *k_norm, *v_norm;
   float eps;
@@ -287,9 +288,10 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Append a) {
         const float2 t = csf[d0 + e];
         v[e] = v[e] * t.x + (first_half ? -partner : partner) * t.y;
       }
-      if (head < a.nq)
-        *reinterpret_cast<u32x4*>(a.q_out + ((int64_t)row * a.nq + head) * HD + sub * 8) =
-            u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+      const u32x4 out = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+      u32x4* to = reinterpret_cast<u32x4*>(a.q_out + ((int64_t)row * a.nq + head) * HD + sub * 8);
+      if (head < a.nq && a.q_past) __builtin_nontemporal_store(out, to);
+      else if (head < a.nq) *to = out;
     } else {
       double v[8];
       x.values(scale, v);
@@ -328,10 +330,13 @@ int kv4_append(const void* qkv, int splits, int B, int W, int nq, int nkv, int h
   // few rows: one unit per wave, so that the chip has work; many: a workgroup per row, which finds the angles once
   // (2048 rows of 40 heads, before V went apart: 18.4 us, 20.3 with a unit per wave)
   const int units_per_wg = rows < 256 ? 4 : (int)qk_units, chunks = (int)ceil_div(qk_units, units_per_wg);
+  // many rows' queries leave the L2 before they are read (2048 rows: 20.6 us kept, 19.3 past it, with the read-back;
+  // followed by its attention, one row 12.8 and 12.95)
+  const int q_past = rows >= 256;
   const int units = nkv * (hd / 128), v_units = rows < 256 ? 4 : units, v_chunks = (int)ceil_div(units, v_units);
   const int64_t v_wgs = (int64_t)B * ((W + 6) / 4) * v_chunks;
   DSK_REQUIRE(v_wgs + rows * chunks <= 0x7fffffff, "%s: %lld rows", who, (long long)rows);
-  Kv4Append a = {qkv, splits, W, nq, nkv, (int)v_wgs, v_chunks, v_units, chunks, units_per_wg, rows * (nq + 2 * nkv) * hd,
+  Kv4Append a = {qkv, splits, W, nq, nkv, (int)v_wgs, v_chunks, v_units, chunks, units_per_wg, q_past, rows * (nq + 2 * nkv) * hd,
                  q_norm, k_norm, v_norm, eps, inv_freq, seq_lens, pos_offset, block_table, max_pages, page, (uint8_t*)k_pool,
                  (uint8_t*)v_pool, k_sb, v_sb, q_out, x_ssq, x_tiles, (float)(x_tiles * 16), x_eps};
   const dim3 grid((unsigned)(v_wgs + rows * chunks)), blk(256);
