@@ -106,6 +106,41 @@ def test_append(dev, nq, nkv, hd, page, B, W, lens, splits, opt):
         assert torch.equal(now.cpu()[~mask], was.cpu()[~mask])
 
 
+@pytest.mark.parametrize("hd,splits,start", [(128, 0, 0), (256, 0, 70001), (128, 3, 130000)])
+def test_append_codes_are_the_nearest(dev, hd, splits, start):
+    """Keys formed in 64 bits: scales, offsets and codes are those of the 64-bit reference, which leaves out values
+    within 1e-7 of a step of the middle between two codes (a 64-bit chain is off by less than 1e-10 of one)."""
+    from mlx_dspark import ops
+
+    nq, nkv, W, page = 2, 2, 300, 64
+    g = torch.Generator().manual_seed(hd + splits)
+    max_pages = -(-(start + W) // page)
+    table = (torch.arange(max_pages, dtype=torch.int32) % 7)[None].to(dev)
+    kp, vp = (torch.zeros((7, nkv, page, hd // 2), dtype=torch.uint8, device=dev) for _ in range(2))
+    ks, vs = (torch.zeros((7, nkv, page, hd // 64), dtype=torch.int32, device=dev) for _ in range(2))
+    x = torch.randn((max(splits, 1), W, (nq + 2 * nkv) * hd), generator=g)
+    x = x if splits else x[0].to(torch.bfloat16)
+    kn = (1 + 0.2 * torch.randn(hd, generator=g)).to(torch.bfloat16)
+    inv = ops.rope_inv_freq(hd, 1e6, "cpu")
+    ops.qkv_rope_append(x.to(dev), 1, W, nq, nkv, hd, kn.to(dev), kn.to(dev), EPS, inv.to(dev),
+                        torch.tensor([start], dtype=torch.int32, device=dev), table, page, ops.DSK_KV_U4, kp, vp, ks, vs)
+    r = (x.double().sum(0) if splits else x.double()).view(W, nq + 2 * nkv, hd)
+    pos = torch.arange(start, start + W)
+    pg, sl = table[0].cpu().long()[pos // page], pos % page
+    for which, pool, sb, want in (("k", kp, ks, _rope64(_norm64(r[:, nq:nq + nkv], kn), pos, inv)), ("v", vp, vs, r[:, nq + nkv:])):
+        if which == "v" and not splits:
+            continue    # bf16 values: float32, as test_append_bf16_values_exact has them
+        w = want.view(W, nkv, -1, 64)
+        lo, hi = w.amin(-1), w.amax(-1)
+        s, b = ((t.float().to(torch.bfloat16)).double() for t in ((hi - lo) / 15, lo))
+        got_s, got_b = (t[pg, :, sl].double() for t in words(sb))
+        assert torch.equal(got_s, s) and torch.equal(got_b, b)
+        near = (w - b[..., None]) / s[..., None]
+        c = decode(pool, sb, hd, which)[0][pg, :, sl].view(W, nkv, -1, 64)
+        sure = ((near - near.floor()) - 0.5).abs() > 1e-7
+        assert torch.equal(c[sure].double(), near.round().clamp(0, 15)[sure])
+
+
 @pytest.mark.parametrize("hd", [128, 256])
 def test_append_bf16_values_exact(dev, hd):
     """V rows of a bf16 projection take no arithmetic before their codes: the float32 rule's own bits, constant
