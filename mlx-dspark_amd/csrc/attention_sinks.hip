@@ -15,11 +15,11 @@
 // range and nothing is lost, and a block costs one vote instead of two lane exchanges and a rescale.
 //
 // Measured, us (the kernel, then with the join of its splits in a graph; rates are of the whole):
-//   4-bit, 32 heads of 128 over 8: one token after 16384 .. 65536 in 4 rows 46, 52: 3.3 TB/s of codes; 16 tokens
+//   4-bit, 32 heads of 128 over 8: one token after 16384 .. 65536 in 4 rows 43, 51: 3.4 TB/s of codes; 16 tokens
 //     after 4096 11.7, 15.5; a prompt of 4096 tokens 268, unsplit: 0.51 PFLOP/s of scores and outputs, 1.03 with the
 //     three terms
-//   8-bit, window 4096 and 64 sinks, one token in 8 rows of 2048 .. 32768 20, 24: 2.7 TB/s
-//   bf16, 16 heads of 256 over 8, window 1024, 9 tokens 12.4, 16
+//   8-bit, window 4096 and 64 sinks, one token in 8 rows of 2048 .. 32768 19, 23.7: 2.8 TB/s
+//   bf16, 16 heads of 256 over 8, window 1024, 9 tokens 12.7, 16
 //   4-bit, the same window, a prompt of 2048 tokens after 1000 102, unsplit: 0.34 PFLOP/s, 0.67 with the terms
 #include <algorithm>
 #include <type_traits>

@@ -13,7 +13,7 @@ namespace dsk {
 // 2048-token prompt are not the nearest (1.4 us more for 40 heads of 128 with 8 of V).
 //
 // What bounds it: few rows, the chain of loads (lengths, row, angles: 6.6 us for one token in a graph, of which
-// about 4 are two launches); many, the bytes: 44 MB for that prompt, 14.4 us, 3.1 TB/s.
+// about 4 are two launches); many, the bytes: 44 MB for that prompt, 14.6 us, 3.0 TB/s.
 //
 // Queries and keys: one workgroup per token row and chunk of heads; the row's HD / 2 sines and cosines are found
 // once, one per thread, for all heads of the chunk; then 8 dims per lane, HD / 8 lanes per head. V, in the same
@@ -354,7 +354,7 @@ int kv4_append(const void* qkv, int splits, int B, int W, int nq, int nkv, int h
 // ----------------------------------------------------------------------------- read back
 // K and V of positions first[b] + offset + i, i < n, as bf16 rows: one workgroup per 32 positions (whole
 // V blocks) of a (row, kv head), 8 dims per thread and step. A copy: bound by the bytes it writes (4-bit codes of
-// 32768 tokens, 8 heads of 128: 28.8 us, 6.0 TB/s read and written; of 1027, 256 dims: 7 us, its chain of loads).
+// 32768 tokens, 8 heads of 128: 28.8 us, 6.0 TB/s read and written; of 1027, 256 dims: 6.2 us, its chain of loads).
 // The stores pass the caches by: with ordinary ones the same call took 50 us once it wrote buffers that no cache held.
 struct KvRead {
   const int32_t* first;
